@@ -81,7 +81,7 @@ int kx_graph_destroy(void* graph_exec);
  * record holds) to the host after a device synchronise; kx_bounds_reset clears the record.  In a
  * normal build kx_bounds_enabled() is 0 and the other two return KX_EUNSUPPORTED.
  * file_id: 1 gemv_w8, 2 gemm_w8_rows, 3 gemm_w8, 4 gemm_f16, 5 attn_decode, 6 attn_prefill,
- * 7 support, 8 gemv_f32, 9 gemv_engine; operand: the index the kernel file gives the buffer; offset: byte offset
+ * 7 support, 8 gemv_f32, 9 gemv_engine, 10 paged_write, 11 paged_decode, 12 prompt_attn, 13 logprobs; operand: the index the kernel file gives the buffer; offset: byte offset
  * of the access from the block's start; extent: the block's size in bytes. */
 typedef struct kx_bounds_record {
   int32_t file_id, line, operand, pad_;
@@ -579,6 +579,155 @@ int kx_fill_hash_i8(int8_t* dst, int32_t rows, int32_t cols, int64_t ld, int64_t
                     uint64_t seed, void* stream);
 int kx_fill_hash_f32(float* dst, int32_t rows, int32_t cols, int64_t ld, int64_t row0,
                      int64_t col0, uint64_t seed, float lo, float hi, void* stream);
+
+/* ---------------- batched serving: a paged KV cache and its operators ----------------
+ * The entries above step one sequence over a cache of consecutive rows, as the reference does
+ * (llama3.cpp:656-743, kv_cache_manager.cpp:6-40).  The entries below serve a batch of sequences of
+ * different lengths in one launch each.  No counterpart in the reference.
+ *
+ * Element types of these entries; bf16 is the upper half of an fp32 value. */
+enum { KX_F32 = 0, KX_F16 = 1, KX_BF16 = 2 };
+
+/* One layer's K and V pages and what says which sequence holds which page.  Row r of page p of kv head
+ * h starts at element p * page_stride + r * row_stride + h * head_stride of `key` and of `value`
+ * ([page][row][kv head][head_size]: row_stride = kv_head_num * head_size, head_stride = head_size;
+ * [page][kv head][row][head_size]: row_stride = head_size, head_stride = page_size * head_size).
+ * Position t of sequence b is row t % page_size of page table[b * table_stride + t / page_size].
+ * table and seq_lens are device memory, read by the kernels: a captured launch is replayed as they
+ * change.  seq_lens[b] counts the rows of sequence b INCLUDING those of the call; a length below zero
+ * counts as zero, one above table_pages * page_size as that.  A table entry outside 0..num_pages-1 is
+ * a page that is not there (one that a sliding window has left behind, say): nothing is read or
+ * written through it and its positions are seen by no query.
+ * head_size 32, 64 or 128 (else KX_EUNSUPPORTED); any page size; strides that are at least head_size and
+ * multiples of 16 bytes, key and value aligned to 16 bytes; page_size * table_pages below 2^31. */
+typedef struct kx_paged_kv {
+  int32_t type;          /* KX_F32 / KX_F16 / KX_BF16 */
+  int32_t kv_head_num, head_size;
+  int32_t page_size, num_pages;
+  int32_t table_pages;   /* entries of a table row */
+  int32_t batch;         /* rows of the table, entries of seq_lens; 0: the call does nothing */
+  void* key;
+  void* value;
+  int64_t page_stride, row_stride, head_stride; /* elements */
+  const int32_t* table;
+  int64_t table_stride;  /* entries from one table row to the next */
+  const int32_t* seq_lens;
+} kx_paged_kv;
+
+/* New rows into the pages, with the RoPE of each row's own position (kx_rope_f32 rotates consecutive
+ * rows from one position; rope_kernel.cu).  The new rows of the batch are packed: rows cu_rows[b] ..
+ * cu_rows[b+1]-1 (device, batch + 1 non-decreasing entries) are the LAST positions of sequence b: row i of its n
+ * sits at position seq_lens[b] - n + i.  k is rotated and filed, v filed as it is, q (nullable) rotated
+ * into q_out, which may be q; all with the tables and pairings of kx_sin_cos_cache_f32 / kx_rope_f32,
+ * in fp32, rounded once to the type of the destination (saturating at +-65504 for fp16).  sin_cache
+ * and cos_cache NULL: no rotation (q and q_out have to be NULL too).  src_type is that of k, v, q and
+ * q_out: KX_F32 into any cache, KX_F16 / KX_BF16 into a cache of the same type.  A row whose position
+ * is outside 0 .. table_pages * page_size - 1, has no page or (when rotating) lies past table_rows is not filed; past
+ * table_rows or below zero its q row is left alone too.  Rows of no sequence (below cu_rows[0], from cu_rows[batch] on) are left
+ * alone.  No two rows of a call may have the same place in the pages.  Strides in elements, multiples of 4 and
+ * at least the row's width; pointers aligned to 16 bytes (KX_EINVAL). */
+typedef struct kx_paged_write_desc {
+  kx_paged_kv kv;
+  int32_t src_type;
+  int32_t rows;            /* rows of k, v and q */
+  int32_t head_num;        /* heads of q */
+  int32_t rope_variant;    /* KX_ROPE_* */
+  int32_t table_rows;      /* rows of the sin/cos tables */
+  const int32_t* cu_rows;
+  const void* k;
+  int64_t k_stride;
+  const void* v;
+  int64_t v_stride;
+  const void* q;
+  int64_t q_stride;
+  void* q_out;
+  int64_t q_out_stride;
+  const float* sin_cache;
+  const float* cos_cache;
+} kx_paged_write_desc;
+int kx_paged_write(const kx_paged_write_desc* desc, void* stream);
+
+/* Attention of one new token per sequence over its pages (kx_mha_decode_f32 for a batch): for head h of
+ * sequence b, over the positions max(0, seq_lens[b] - window) <= t < seq_lens[b] (window 0: all),
+ *   out[b][h] = sum_t softmax_t(scale * q[b][h] . K_b[t][h / (head_num / kv_head_num)]) * V_b[t][..]
+ * in fp32 arithmetic; zeros where no position is seen.  q and out rows of head_num * head_size at their
+ * strides (elements, multiples of 16 bytes), of type q_type: KX_F32 over any cache, KX_F16 / KX_BF16 over
+ * a cache of the same type.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
+ * must be ZERO before its first use and is left ready for the next call by every call; calls that
+ * share one must not overlap in time (kx_attn_workspace_reset's rule: after an aborted launch clear it again).
+ * The lengths are read by the kernel, which cuts the batch's keys evenly over the chip. */
+typedef struct kx_paged_decode_desc {
+  kx_paged_kv kv;
+  int32_t q_type;
+  int32_t head_num;
+  int32_t window;
+  float scale;
+  const void* q;
+  int64_t q_stride;
+  void* out;
+  int64_t out_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} kx_paged_decode_desc;
+size_t kx_paged_decode_workspace_bytes(int32_t batch, int32_t head_num, int32_t kv_head_num, int32_t head_size);
+int kx_paged_decode(const kx_paged_decode_desc* desc, void* stream);
+
+/* Attention of packed prompts of different lengths (kx_flash_attention_f32 for a batch): query rows
+ * cu_q[b] .. cu_q[b+1]-1 of sequence b attend its key rows, cu_k[b] .. cu_k[b+1]-1 of k and v (device,
+ * batch + 1 non-decreasing entries each; cu_k may be cu_q), or with `pages` (host pointer; k, v, cu_k NULL then) positions 0 ..
+ * seq_lens[b]-1 of the pages.  The last query row stands at the last key: row i of n at position
+ * p = (keys - n) + i; causal: it sees the keys t <= p, with window > 0 (causal only) of these t > p - window.
+ * A row that sees nothing gets zeros; rows of no sequence are left alone.  All of one type
+ * (KX_F16 / KX_BF16: matrix-core products of that type with fp32 sums and softmax, probabilities
+ * rounded to it for the second product; KX_F32: fp32 throughout).  head_size 32, 64 or 128.  Strides in elements (q and
+ * out: head_num * head_size or more, k and v: kv_head_num * head_size or more), multiples of 16 bytes. */
+typedef struct kx_prompt_attn_desc {
+  int32_t type;
+  int32_t head_num, kv_head_num, head_size;
+  int32_t batch;
+  int32_t q_rows, k_rows;  /* rows of q and out, of k and v */
+  int32_t causal, window;
+  float scale;
+  const void* q;
+  int64_t q_stride;
+  const void* k;
+  int64_t k_stride;
+  const void* v;
+  int64_t v_stride;
+  void* out;
+  int64_t out_stride;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const kx_paged_kv* pages;
+} kx_prompt_attn_desc;
+int kx_prompt_attention(const kx_prompt_attn_desc* desc, void* stream);
+
+/* What an answer says about its tokens (kx_argmax_f32 for more than the first): per row of logits
+ *   logprob[r] = x[tokens[r]] - log sum_v e^{x[v]}            (tokens, logprob: both or neither NULL)
+ *   entropy[r] = - sum_v p[v] log p[v], a banned (-inf) logit adding nothing      (nullable)
+ *   top_ids / top_logprobs [rows][top_n]: the top_n largest in falling order, the lower index ahead
+ *     among equal ones; NaN ranks below -inf         (top_n 0: NULL; top_n <= min(vocab, KX_LOGPROBS_TOP_MAX))
+ * in fp32.  A token below zero is none: logprob 0; one past the vocabulary: NaN.  A row that is no
+ * distribution (holds NaN or +inf, or nothing but -inf) gives NaN for the three kinds of numbers, and its ids in order.
+ * Logits of `type`, rows at row_stride elements (any, >= vocab), aligned to their element.  workspace as for
+ * kx_paged_decode, of kx_token_logprobs_workspace_bytes(rows, vocab, top_n) bytes. */
+#define KX_LOGPROBS_TOP_MAX 32
+typedef struct kx_logprobs_desc {
+  int32_t type;
+  int32_t rows, vocab;
+  int32_t top_n;
+  const void* logits;
+  int64_t row_stride;
+  const int32_t* tokens;
+  float* logprob;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+  void* workspace;
+  size_t workspace_bytes;
+} kx_logprobs_desc;
+size_t kx_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_n);
+int kx_token_logprobs(const kx_logprobs_desc* desc, void* stream);
 
 /* ---------------- tensor-parallel communicator ----------------
  * Replaces NcclHandler (kuiper/include/base/nccl_handler.h:29-58, source/base/nccl_handler.cpp:

@@ -17,6 +17,8 @@ LIB_PATH = os.environ.get("KX_HIP_LIB") or os.path.join(LIB_DIR, "libkx_hip.so")
 ROPE_INTERLEAVED = 0
 ROPE_HALF_SPLIT = 1
 
+F32, F16, BF16 = 0, 1, 2  # KX_F32 / KX_F16 / KX_BF16
+
 
 class KxError(RuntimeError):
     pass
@@ -151,6 +153,12 @@ SIGNATURES = {
     "kx_fill_hash_i8": (C.c_int, [_vp, _i32, _i32, C.c_int64, C.c_int64, C.c_int64, C.c_uint64, _vp]),
     "kx_fill_hash_f32": (C.c_int, [_vp, _i32, _i32, C.c_int64, C.c_int64, C.c_int64, C.c_uint64, _f,
                                    _f, _vp]),
+    "kx_paged_write": (C.c_int, [_vp, _vp]),
+    "kx_paged_decode_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "kx_paged_decode": (C.c_int, [_vp, _vp]),
+    "kx_prompt_attention": (C.c_int, [_vp, _vp]),
+    "kx_token_logprobs_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "kx_token_logprobs": (C.c_int, [_vp, _vp]),
     "kx_comm_unique_id": (C.c_int, [_vp]),
     "kx_comm_init_rank": (C.c_int, [C.POINTER(_vp), _vp, _i32, _i32]),
     "kx_comm_destroy": (C.c_int, [_vp]),
@@ -181,6 +189,49 @@ class GemvDesc(C.Structure):
 GEMV_PLAIN, GEMV_GATE_UP, GEMV_QKV_ROPE = 0, 1, 2
 
 
+class PagedKv(C.Structure):
+    """kx_paged_kv of include/kx_hip.h, field for field."""
+    _fields_ = [("type", C.c_int32), ("kv_head_num", C.c_int32), ("head_size", C.c_int32),
+                ("page_size", C.c_int32), ("num_pages", C.c_int32), ("table_pages", C.c_int32),
+                ("batch", C.c_int32), ("key", C.c_void_p), ("value", C.c_void_p), ("page_stride", C.c_int64),
+                ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("seq_lens", C.c_void_p)]
+
+
+class PagedWriteDesc(C.Structure):
+    """kx_paged_write_desc, field for field."""
+    _fields_ = [("kv", PagedKv), ("src_type", C.c_int32), ("rows", C.c_int32), ("head_num", C.c_int32),
+                ("rope_variant", C.c_int32), ("table_rows", C.c_int32), ("cu_rows", C.c_void_p), ("k", C.c_void_p),
+                ("k_stride", C.c_int64), ("v", C.c_void_p), ("v_stride", C.c_int64), ("q", C.c_void_p),
+                ("q_stride", C.c_int64), ("q_out", C.c_void_p), ("q_out_stride", C.c_int64),
+                ("sin_cache", C.c_void_p), ("cos_cache", C.c_void_p)]
+
+
+class PagedDecodeDesc(C.Structure):
+    """kx_paged_decode_desc, field for field."""
+    _fields_ = [("kv", PagedKv), ("q_type", C.c_int32), ("head_num", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float), ("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p),
+                ("out_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class PromptAttnDesc(C.Structure):
+    """kx_prompt_attn_desc, field for field (pages: the address of a PagedKv that outlives the call)."""
+    _fields_ = [("type", C.c_int32), ("head_num", C.c_int32), ("kv_head_num", C.c_int32), ("head_size", C.c_int32),
+                ("batch", C.c_int32), ("q_rows", C.c_int32), ("k_rows", C.c_int32), ("causal", C.c_int32),
+                ("window", C.c_int32), ("scale", C.c_float), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("k", C.c_void_p), ("k_stride", C.c_int64), ("v", C.c_void_p), ("v_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p),
+                ("pages", C.c_void_p)]
+
+
+class LogprobsDesc(C.Structure):
+    """kx_logprobs_desc, field for field."""
+    _fields_ = [("type", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("top_n", C.c_int32),
+                ("logits", C.c_void_p), ("row_stride", C.c_int64), ("tokens", C.c_void_p), ("logprob", C.c_void_p),
+                ("entropy", C.c_void_p), ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class BoundsRecord(C.Structure):
     """kx_bounds_record of include/kx_hip.h."""
     _fields_ = [("file_id", C.c_int32), ("line", C.c_int32), ("operand", C.c_int32), ("pad_", C.c_int32),
@@ -189,7 +240,8 @@ class BoundsRecord(C.Structure):
 
 BOUNDS_FILES = {1: "gemv_w8.hip", 2: "gemm_w8_rows.hip", 3: "gemm_w8.hip", 4: "gemm_f16.hip",
                 5: "attn_decode.hip", 6: "attn_prefill.hip", 7: "support.hip", 8: "gemv_f32.hip",
-                9: "gemv_engine.hip"}
+                9: "gemv_engine.hip", 10: "paged_write.hip", 11: "paged_decode.hip", 12: "prompt_attn.hip",
+                13: "logprobs.hip"}
 
 
 def bounds_enabled():
@@ -544,3 +596,141 @@ def gemv_chain(descs, workspace, chain_id=0, pos_dev=None, pos=0, stream=None):
     arr = (GemvDesc * len(descs))(*descs)
     check(lib().kx_gemv_w8_chain_f32(arr, len(descs), workspace.ptr, workspace.nbytes, chain_id, pos_dev, pos,
                                      stream), "kx_gemv_w8_chain_f32")
+
+
+# ---------------- batched serving: paged cache, packed prompts, log probabilities ----------------
+def to_kind(a, kind):
+    """fp32 values as an array of the element type KX_F32 / KX_F16 / KX_BF16 (bf16: uint16 bit patterns,
+    rounded to nearest even)."""
+    a = np.ascontiguousarray(a, np.float32)
+    if kind == F32:
+        return a
+    if kind == F16:
+        return a.astype(np.float16)
+    bits = a.view(np.uint32)
+    rounded = ((bits + (0x7FFF + ((bits >> 16) & 1))) >> 16).astype(np.uint16)
+    return np.where(np.isnan(a), np.uint16(0x7FC0), rounded)
+
+
+def from_kind(a, kind):
+    """An array of an element type as fp32 (exact)."""
+    if kind == BF16:
+        return (a.astype(np.uint32) << 16).view(np.float32)
+    return a.astype(np.float32)
+
+
+KIND_DTYPE = {F32: np.float32, F16: np.float16, BF16: np.uint16}
+
+
+class PagePool:
+    """One layer's pages on the device: key and value [num_pages][page_size][kv_heads][head_size] (or, head_major,
+    [num_pages][kv_heads][page_size][head_size]) fp32 arrays that are rounded to `kind`."""
+
+    def __init__(self, key, value, kind=F32, head_major=False):
+        self.kind, self.head_major, self.shape = kind, head_major, key.shape
+        order = (0, 2, 1, 3) if head_major else (0, 1, 2, 3)
+        self.key = Buf.from_numpy(to_kind(key.transpose(order), kind))
+        self.value = Buf.from_numpy(to_kind(value.transpose(order), kind))
+
+    def desc(self, table, seq_lens):
+        """kx_paged_kv over device buffers: table int32 [batch][table_pages], seq_lens int32 [batch]."""
+        pages, size, heads, hs = self.shape
+        return PagedKv(type=self.kind, kv_head_num=heads, head_size=hs, page_size=size, num_pages=pages,
+                       table_pages=table.shape[1], batch=table.shape[0], key=self.key.ptr, value=self.value.ptr,
+                       page_stride=size * heads * hs, row_stride=hs if self.head_major else heads * hs,
+                       head_stride=size * hs if self.head_major else hs, table=table.ptr,
+                       table_stride=table.shape[1], seq_lens=seq_lens.ptr)
+
+    def read(self):
+        """(key, value) as fp32 [num_pages][page_size][kv_heads][head_size]."""
+        pages, size, heads, hs = self.shape
+        shape = (pages, heads, size, hs) if self.head_major else self.shape
+        out = [from_kind(b.numpy(KIND_DTYPE[self.kind], shape), self.kind) for b in (self.key, self.value)]
+        return [a.transpose(0, 2, 1, 3) if self.head_major else a for a in out]
+
+
+def paged_write(pool, table, seq_lens, cu_rows, k, v, q=None, rope=None, variant=ROPE_HALF_SPLIT, src_kind=F32,
+                in_place=False, stream=None):
+    """kx_paged_write: k, v [rows][kv_heads][hs], q [rows][heads][hs] fp32 arrays (rounded to src_kind), rope:
+    (sin, cos) tables [positions][hs] or None.  Returns the rotated q as fp32 (None without q)."""
+    tb, sl, cu = (Buf.from_numpy(np.asarray(a, np.int32)) for a in (table, seq_lens, cu_rows))
+    rows, heads = k.shape[0], 0 if q is None else q.shape[1]
+    dk, dv = Buf.from_numpy(to_kind(k, src_kind)), Buf.from_numpy(to_kind(v, src_kind))
+    d = PagedWriteDesc(kv=pool.desc(tb, sl), src_type=src_kind, rows=rows, head_num=heads, rope_variant=variant,
+                       cu_rows=cu.ptr, k=dk.ptr, k_stride=k.shape[1] * k.shape[2], v=dv.ptr,
+                       v_stride=v.shape[1] * v.shape[2])
+    keep = []
+    if rope is not None:
+        keep = [Buf.from_numpy(np.asarray(t, np.float32)) for t in rope]
+        d.sin_cache, d.cos_cache, d.table_rows = keep[0].ptr, keep[1].ptr, rope[0].shape[0]
+    if q is not None:
+        dq = Buf.from_numpy(to_kind(q, src_kind))
+        qo = dq if in_place else Buf.zeros(q.shape, KIND_DTYPE[src_kind])
+        d.q, d.q_stride, d.q_out, d.q_out_stride = dq.ptr, heads * q.shape[2], qo.ptr, heads * q.shape[2]
+    check(lib().kx_paged_write(C.byref(d), stream), "kx_paged_write")
+    sync()
+    return None if q is None else from_kind(qo.numpy(KIND_DTYPE[src_kind], q.shape), src_kind)
+
+
+def paged_decode(pool, table, seq_lens, q, scale=None, window=0, q_kind=F32, workspace=None, stream=None):
+    """kx_paged_decode: q [batch][heads][hs] fp32 (rounded to q_kind); returns [batch][heads][hs] as fp32.
+    workspace: a zero-filled Buf that earlier calls may have used."""
+    batch, heads, hs = q.shape
+    tb, sl = (Buf.from_numpy(np.asarray(a, np.int32)) for a in (table, seq_lens))
+    dq, out = Buf.from_numpy(to_kind(q, q_kind)), Buf.zeros(q.shape, KIND_DTYPE[q_kind])
+    if workspace is None:
+        workspace = Buf.zeros(lib().kx_paged_decode_workspace_bytes(batch, heads, pool.shape[2], hs), np.uint8)
+    d = PagedDecodeDesc(kv=pool.desc(tb, sl), q_type=q_kind, head_num=heads, window=window,
+                        scale=1.0 / np.sqrt(hs) if scale is None else scale, q=dq.ptr, q_stride=heads * hs,
+                        out=out.ptr, out_stride=heads * hs, workspace=workspace.ptr, workspace_bytes=workspace.nbytes)
+    check(lib().kx_paged_decode(C.byref(d), stream), "kx_paged_decode")
+    sync()
+    return from_kind(out.numpy(KIND_DTYPE[q_kind], q.shape), q_kind)
+
+
+def prompt_attention(q, cu_q, k=None, v=None, cu_k=None, pool=None, table=None, seq_lens=None, kv_heads=None,
+                     causal=True, window=0, scale=None, kind=F16, fill=0.0, stream=None):
+    """kx_prompt_attention over packed rows k, v [rows][kv_heads][hs], or over a PagePool with its table and
+    lengths; q [rows][heads][hs].  fp32 arrays, rounded to `kind`; returns [rows][heads][hs] as fp32.  fill: what
+    the output holds before the call."""
+    rows, heads, hs = q.shape
+    cu = Buf.from_numpy(np.asarray(cu_q, np.int32))
+    dq, out = Buf.from_numpy(to_kind(q, kind)), Buf.from_numpy(to_kind(np.full(q.shape, fill), kind))
+    d = PromptAttnDesc(type=kind, head_num=heads, head_size=hs, batch=len(cu_q) - 1, q_rows=rows,
+                       causal=1 if causal else 0, window=window, scale=1.0 / np.sqrt(hs) if scale is None else scale,
+                       q=dq.ptr, q_stride=heads * hs, out=out.ptr, out_stride=heads * hs, cu_q=cu.ptr)
+    if pool is not None:
+        tb, sl = (Buf.from_numpy(np.asarray(a, np.int32)) for a in (table, seq_lens))
+        pages = pool.desc(tb, sl)
+        d.kv_head_num, d.pages = pool.shape[2], C.addressof(pages)
+    else:
+        dk, dv = Buf.from_numpy(to_kind(k, kind)), Buf.from_numpy(to_kind(v, kind))
+        ck = Buf.from_numpy(np.asarray(cu_q if cu_k is None else cu_k, np.int32))
+        d.kv_head_num, d.k, d.v, d.cu_k, d.k_rows = k.shape[1], dk.ptr, dv.ptr, ck.ptr, k.shape[0]
+        d.k_stride = d.v_stride = k.shape[1] * hs
+    check(lib().kx_prompt_attention(C.byref(d), stream), "kx_prompt_attention")
+    sync()
+    return from_kind(out.numpy(KIND_DTYPE[kind], q.shape), kind)
+
+
+def token_logprobs(logits, tokens=None, top_n=0, kind=F32, entropy=True, row_stride=None, workspace=None, stream=None):
+    """kx_token_logprobs: logits [rows][vocab] fp32 (rounded to `kind`).  Returns (logprob or None, entropy or
+    None, top_ids, top_logprobs), the last two [rows][top_n]."""
+    rows, vocab = logits.shape
+    row_stride = row_stride or vocab
+    wide = np.zeros((rows, row_stride), np.float32)
+    wide[:, :vocab] = logits
+    dl = Buf.from_numpy(to_kind(wide, kind))
+    dt = None if tokens is None else Buf.from_numpy(np.asarray(tokens, np.int32))
+    lp, en = Buf.zeros(rows), Buf.zeros(rows)
+    ids, tl = Buf.zeros((rows, max(top_n, 1)), np.int32), Buf.zeros((rows, max(top_n, 1)))
+    if workspace is None:
+        workspace = Buf.zeros(lib().kx_token_logprobs_workspace_bytes(rows, vocab, top_n), np.uint8)
+    d = LogprobsDesc(type=kind, rows=rows, vocab=vocab, top_n=top_n, logits=dl.ptr, row_stride=row_stride,
+                     tokens=None if dt is None else dt.ptr, logprob=None if dt is None else lp.ptr,
+                     entropy=en.ptr if entropy else None, top_ids=ids.ptr if top_n else None,
+                     top_logprobs=tl.ptr if top_n else None, workspace=workspace.ptr, workspace_bytes=workspace.nbytes)
+    check(lib().kx_token_logprobs(C.byref(d), stream), "kx_token_logprobs")
+    sync()
+    return (None if dt is None else lp.numpy(), en.numpy() if entropy else None,
+            ids.numpy(np.int32, (rows, max(top_n, 1)))[:, :top_n], tl.numpy(np.float32, (rows, max(top_n, 1)))[:, :top_n])
