@@ -655,7 +655,8 @@ int kx_paged_write(const kx_paged_write_desc* desc, void* stream);
  * a cache of the same type.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
  * must be ZERO before its first use and is left ready for the next call by every call; calls that
  * share one must not overlap in time (kx_attn_workspace_reset's rule: after an aborted launch clear it again).
- * The lengths are read by the kernel, which cuts the batch's keys evenly over the chip. */
+ * The lengths are read by the kernel, which cuts the batch's keys evenly over the chip.  KX_EUNSUPPORTED for more
+ * than 1024 kv heads (a kv head of more than 16 query heads counts once per 16). */
 typedef struct kx_paged_decode_desc {
   kx_paged_kv kv;
   int32_t q_type;
