@@ -7,10 +7,18 @@ namespace kx {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
-template <int KIND> struct KindOf;
-template <> struct KindOf<KX_F32> { typedef float type; };
-template <> struct KindOf<KX_F16> { typedef _Float16 type; };
-template <> struct KindOf<KX_BF16> { typedef __bf16 type; };
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive prefix sum over the 64 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+  return v;
+}
 
 // Four / eight consecutive elements, widened exactly.
 __device__ __forceinline__ void load4(const float* p, float (&o)[4]) {

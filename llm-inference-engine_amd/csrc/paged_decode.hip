@@ -28,9 +28,6 @@
 
 namespace kx {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-
 enum DecodeOperand { PD_KEY, PD_VALUE, PD_TABLE, PD_LENS, PD_Q, PD_OUT, PD_WS };
 
 constexpr int kPdWaves = 4;
@@ -50,17 +47,6 @@ struct PagedDecodeArgs {
   float scale;
   KX_BFIELD(7)
 };
-
-// ---- wave-wide integer helpers ----
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive prefix sum over the 64 lanes
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
-  return v;
-}
 
 // What a workgroup works on.
 struct DecodeWork {

@@ -1,56 +1,494 @@
 // Attention of packed prompts of different lengths, keys and values packed beside them or in pages.
+//
+//   row i of n at position p = (keys - n) + i:  s_t = scale q_i . k_t,  out_i = sum_t e^{s_t - m} v_t / sum_t e^{s_t - m}
+//   over the t that it sees: t < keys, t <= p when causal, t > p - window with a window.
+//
+// Bound: 4 hs operations per (head, row, seen key) on the matrix cores; K and V come from L2.
+//
+// Split: the rows of a sequence times the kv_mul query heads of a kv head are one list of (row, head) pairs; a
+// workgroup takes 32 consecutive pairs per wave, so any grouping of heads fills the tiles and a staged K/V tile
+// feeds all heads that share it.  A workgroup finds its sequence by a prefix sum over the lengths: no plan from the host.
+//
+// Tile: 64 keys in LDS, two buffers, filled by LDS-DMA (a wave instruction moves 1 KiB, every lane from an address of
+// its own, so rows may come from pages), one barrier per tile.  A row's 16-byte pieces sit exclusive-or-ed with a
+// row key, applied to the source address and to the reads, which makes both products' reads conflict-free.
+//
+// Products: S^T = K Q^T leaves the keys on the register axis and the pair on the lane, so the softmax state is one
+// value per lane and the weights are already the B operand of O^T = V^T P^T; the A operand V^T comes out of row-major V by
+// transposing LDS reads (16-bit types), or one element per lane (fp32).
+//
+// Rounding: products of 16-bit operands are exact in fp32 and summed there, softmax in fp32, weights rounded to the
+// type for the second product, the sum of the weights unrounded.  The running maximum follows only when it is
+// exceeded by more than 2^8: weights up to 256 have the same relative precision, and the rescaling pass is rare.
 #include <math.h>
 
+#include <type_traits>
+
 #define KX_FILE_ID 12
-#include "attn_simple.hpp"
+#include "paged.hpp"
 
 namespace kx {
 
+enum PromptOperand { PP_Q, PP_K, PP_V, PP_OUT, PP_CUQ, PP_CUK, PP_TABLE, PP_LENS };
+
+constexpr int kPaKeys = 64;  // keys per tile
+
+enum { PA_PACKED = 0, PA_BLOCK_PAGES = 1, PA_ANY_PAGES = 2 };  // where rows are: see row sources below
+
 struct PromptArgs {
-  PagedView kv;  // table: null for packed keys
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
+  PagedView kv;
+  const char* q;
+  const char* k;  // packed rows, or the pages
+  const char* v;
+  char* out;
   const int32_t* cu_q;
   const int32_t* cu_k;
   int64_t q_stride, k_stride, v_stride, out_stride;
-  int32_t batch, head_num, kv_heads, head_size, q_rows, k_rows, causal, window;
+  int32_t batch, kv_heads, kv_mul, q_rows, k_rows, causal, window;
+  PageDiv mul_div;  // division by kv_mul
   float scale;
+  KX_BFIELD(8)
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void prompt_attn_simple_kernel(const PromptArgs a) {
-  const int h = blockIdx.x, row = blockIdx.y, kvh = h / (a.head_num / a.kv_heads);
-  if (a.cu_q[0] > row || a.cu_q[a.batch] <= row) return;
-  int b = 0, up = a.batch;
-  while (up - b > 1) {
-    const int mid = (b + up) >> 1;
-    if (a.cu_q[mid] <= row) b = mid;
-    else up = mid;
+// A workgroup's part of the batch.
+struct PromptWork {
+  int b, q0, n;      // sequence, its first row in q, its rows
+  int k0, keys;      // first key row (packed), keys
+  int block;         // 32 * waves pairs from here
+};
+
+__device__ __forceinline__ int clamp_row(int x, int rows) { return min(max(x, 0), rows); }
+
+template <int ROWS, bool PAGED>
+__device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, PromptWork& w) {
+  const int lane = lane_id();
+  int done = 0;
+  for (int base = 0; base < a.batch; base += 64) {
+    const int b = base + lane;
+    int q0 = 0, n = 0;
+    if (b < a.batch) {
+      q0 = clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b), a.q_rows);
+      n = max(clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b + 1), a.q_rows) - q0, 0);
+    }
+    const int blocks = (int)(((int64_t)n * a.kv_mul + ROWS - 1) / ROWS);
+    const int upto = wave_scan(blocks);
+    const unsigned long long past = __ballot(done + upto > item);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      w.b = base + l;
+      w.q0 = __builtin_amdgcn_readlane(q0, l);
+      w.n = __builtin_amdgcn_readlane(n, l);
+      // a sequence's last blocks first: they see the most keys
+      w.block = done + __builtin_amdgcn_readlane(upto, l) - 1 - item;
+      if (PAGED) {
+        w.k0 = 0;
+        w.keys = min(max(*KX_CK(a, PP_LENS, a.kv.seq_lens + w.b), 0), a.kv.capacity());
+      } else {
+        w.k0 = clamp_row(*KX_CK(a, PP_CUK, a.cu_k + w.b), a.k_rows);
+        w.keys = max(clamp_row(*KX_CK(a, PP_CUK, a.cu_k + w.b + 1), a.k_rows) - w.k0, 0);
+      }
+      return true;
+    }
+    done += __builtin_amdgcn_readlane(upto, 63);
   }
-  int k0 = 0, keys;
-  if (a.kv.table) {
-    keys = min(max(a.kv.seq_lens[b], 0), a.kv.capacity());
-  } else {
-    k0 = min(max(a.cu_k[b], 0), a.k_rows);
-    keys = max(min(a.cu_k[b + 1], a.k_rows) - k0, 0);
+  return false;
+}
+
+// The 16-byte piece of a K (V) row that sits at position c of its place in LDS is c ^ key.  K rows are read 16 at a
+// time at one piece: the 16 positions cover the banks once.  V rows: 4 (16-bit) rows x 64 bytes at a time,
+// or two rows four apart x 128 bytes (fp32).
+template <int CH>
+__device__ __forceinline__ int k_swizzle(int row) { return CH >= 16 ? row % 16 : CH == 8 ? row / 2 % 8 : row / 4 % 4; }
+template <int CH, bool F32>
+__device__ __forceinline__ int v_swizzle(int row) {
+  if (F32) return CH >= 16 ? (row >> 2 & 1) << 3 : 0;
+  return CH == 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0;
+}
+
+template <typename T> struct PromptMma;
+template <> struct PromptMma<_Float16> {
+  typedef f16x8 frag;
+  static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  const int p = keys - a.cu_q[b + 1] + row;  // position of the row
-  const int hi = a.causal ? min(p + 1, keys) : keys;
-  const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
-  const int32_t* table = a.kv.table + b * a.kv.table_stride;
-  auto row_of = [&](int t, bool value) -> const T* {
-    if (!a.kv.table)
-      return value ? static_cast<const T*>(a.v) + (k0 + t) * a.v_stride + kvh * a.head_size
-                   : static_cast<const T*>(a.k) + (k0 + t) * a.k_stride + kvh * a.head_size;
-    const int col = a.kv.div.page(t), page = table[col];
-    if (page < 0 || page >= a.kv.num_pages) return nullptr;
-    return reinterpret_cast<const T*>(value ? a.kv.value : a.kv.key) + page * a.kv.page_stride +
-           (t - col * a.kv.div.size) * a.kv.row_stride + kvh * a.kv.head_stride;
+};
+template <> struct PromptMma<__bf16> {
+  typedef bf16x8 frag;
+  static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct PromptMma<float> { typedef f32x4 frag; };
+
+template <typename T, int HS, int MODE, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArgs a) {
+  constexpr bool F32 = sizeof(T) == 4, PAGED = MODE != PA_PACKED;
+  constexpr int ROWB = HS * (int)sizeof(T);      // bytes of a row
+  constexpr int CH = ROWB / 16;                  // its pieces
+  constexpr int RPP = 1024 / ROWB;               // rows per DMA instruction
+  constexpr int TILEB = kPaKeys * ROWB;          // K (or V) bytes of a tile
+  constexpr int KP = TILEB / 1024;               // DMA instructions for them
+  constexpr int PER = 2 * KP / NW;               // per wave
+  constexpr int DT = HS / 32;                    // output tiles
+  // fp16 weights are held 2^7 times as large: at most 2^15, and whole down to 2^-21 of the largest
+  constexpr float kShift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
+  constexpr int KS = HS * (int)sizeof(T) / 32;   // 32-byte steps of the first product
+  static_assert(2 * KP % NW == 0, "");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers: K tile, V tile
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  typedef const __attribute__((address_space(3))) char* lds_bytes;
+
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int qcol = lane & 31, half = lane >> 5;
+  const int kvh = blockIdx.x % a.kv_heads;
+  PromptWork w;
+  if (!find_prompt<NW * 32, PAGED>(a, blockIdx.x / a.kv_heads, w)) return;
+
+  // ---- this workgroup's and this wave's pairs, and what they see ----
+  const int pairs = w.n * a.kv_mul, f0 = w.block * NW * 32;
+  const int p0 = w.keys - w.n;  // position of row 0, below zero with fewer keys than rows
+  auto hi_of = [&](int row) { return a.causal ? max(min(p0 + row + 1, w.keys), 0) : w.keys; };
+  auto lo_of = [&](int row) { return a.window > 0 ? max(p0 + row - a.window + 1, 0) : 0; };
+  auto row_of = [&](int f) { return a.mul_div.page(min(f, pairs - 1)); };
+  const int hi = hi_of(row_of(f0 + NW * 32 - 1)), lo = min(lo_of(row_of(f0)), hi);
+  const int t0 = lo / kPaKeys, t1 = hi > lo ? (hi + kPaKeys - 1) / kPaKeys : t0;
+  const int wf0 = f0 + wave * 32;
+  const int first_row = row_of(wf0), last_row = row_of(wf0 + 31);
+  const int w_hi = wf0 < pairs ? hi_of(last_row) : 0, w_lo = lo_of(first_row);
+  const int full_hi = hi_of(first_row), full_lo = lo_of(last_row);  // every pair of the wave sees these keys
+  const int my_f = min(wf0 + qcol, pairs - 1), my_row = row_of(my_f), my_head = my_f - my_row * a.kv_mul;
+  const int my_hi = hi_of(my_row), my_lo = lo_of(my_row);
+
+  // ---- row sources ----
+  const int64_t k_stride = PAGED ? a.kv.row_stride : a.k_stride, v_stride = PAGED ? a.kv.row_stride : a.v_stride;
+  const T* kbase = reinterpret_cast<const T*>(a.k) + (PAGED ? kvh * a.kv.head_stride : w.k0 * a.k_stride + kvh * HS);
+  const T* vbase = reinterpret_cast<const T*>(a.v) + (PAGED ? kvh * a.kv.head_stride : w.k0 * a.v_stride + kvh * HS);
+  const int32_t* table = PAGED ? a.kv.table + w.b * a.kv.table_stride : nullptr;
+  auto page_ok = [&](int p) { return (unsigned)p < (unsigned)a.kv.num_pages; };
+  auto lookup = [&](int t) { return *KX_CK(a, PP_TABLE, table + a.kv.div.page(t)); };
+  auto paged_row = [&](const T* base, int page, int t) {
+    return base + (page_ok(page) ? page : 0) * a.kv.page_stride + (t - a.kv.div.page(t) * a.kv.div.size) * a.kv.row_stride;
   };
-  attn_row_simple<T, T>(static_cast<const T*>(a.q) + row * a.q_stride + h * a.head_size,
-                        static_cast<T*>(a.out) + row * a.out_stride + h * a.head_size, a.head_size, lo, hi, a.scale, row_of);
+  // piece i of this wave: rows 16-byte pieces of K (q < KP) or V; a lane's row in the tile and its piece of the row
+  auto piece_row = [&](int i) { return (wave + NW * i) % KP * RPP + lane / CH; };
+  auto piece_is_k = [&](int i) { return wave + NW * i < KP; };
+  unsigned off[PER];  // byte offset of the lane's piece from the tile's first row (packed), or in its row (pages)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int row = piece_row(i);
+    const int c = lane % CH ^ (piece_is_k(i) ? k_swizzle<CH>(row) : v_swizzle<CH, F32>(row));
+    off[i] = 16u * c + (PAGED ? 0u : (unsigned)(row * (int)(piece_is_k(i) ? k_stride : v_stride) * (int)sizeof(T)));
+  }
+  // pages of the next tile's pieces: one per piece where pages are whole 16-row blocks, else one per lane
+  int ids[PAGED ? PER : 1];
+  auto get_ids = [&](int t) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if constexpr (MODE == PA_BLOCK_PAGES)
+          ids[i] = __builtin_amdgcn_readfirstlane(
+              lookup(min(t * kPaKeys + (wave + NW * i) % KP * RPP, (w.keys - 1) & ~(RPP - 1))));
+        else
+          ids[i] = lookup(min(t * kPaKeys + piece_row(i), w.keys - 1));
+      }
+    }
+  };
+  auto issue_tile = [&](int t, int buf) {
+    const int key0 = t * kPaKeys;
+    const bool whole = key0 + kPaKeys <= w.keys;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool is_k = piece_is_k(i);
+      const T* base = is_k ? kbase : vbase;
+      const char* src;
+      if constexpr (PAGED) {
+        int key = key0 + piece_row(i);
+        if (!whole) {  // rows behind the last are replaced by it, within the page of its block
+          if (MODE == PA_BLOCK_PAGES) key = min(key0 + (wave + NW * i) % KP * RPP, (w.keys - 1) & ~(RPP - 1)) + lane / CH;
+          key = min(key, w.keys - 1);
+        }
+        src = reinterpret_cast<const char*>(paged_row(base, ids[i], key)) + off[i];
+      } else {
+        const int64_t stride = is_k ? k_stride : v_stride;
+        const char* tile = reinterpret_cast<const char*>(base + (int64_t)key0 * stride);
+        if (whole) src = tile + off[i];
+        else src = tile + off[i] - (int64_t)max(piece_row(i) - (w.keys - 1 - key0), 0) * stride * (int)sizeof(T);
+      }
+      __builtin_amdgcn_global_load_lds(KX_CKN(a, is_k ? PP_K : PP_V, src, 16),
+                                       (lds_ptr)(smem + buf * 2 * TILEB + (wave + NW * i) * 1024), 16, 0, 0);
+    }
+  };
+
+  if (t0 < t1) {
+    get_ids(t0);
+    issue_tile(t0, 0);
+    if (t0 + 1 < t1) get_ids(t0 + 1);
+  }
+  // a page that is not there: looked for once, and tile by tile only if there is one
+  bool missing = false;
+  if constexpr (PAGED) {
+    if (t0 < t1) {
+      const int c1 = a.kv.div.page(hi - 1);
+      for (int c = a.kv.div.page(lo) + (int)threadIdx.x; c <= c1; c += NW * 64) missing |= !page_ok(*KX_CK(a, PP_TABLE, table + c));
+    }
+    missing = __syncthreads_or(missing);
+  }
+
+  // ---- queries: lane (pair, half) holds the pieces of its row that meet its pieces of a K row ----
+  typedef typename PromptMma<T>::frag frag;
+  frag qf[KS];
+  const T* qrow = reinterpret_cast<const T*>(a.q) + (w.q0 + my_row) * a.q_stride + (kvh * a.kv_mul + my_head) * HS;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    qf[ks] = *KX_CK(a, PP_Q, reinterpret_cast<const frag*>(reinterpret_cast<const char*>(qrow) + 32 * ks + 16 * half));
+  // scores in powers of two; a negative scale turns the queries' sign, and a scale of zero still hides (-inf * 0 is NaN)
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = -qf[ks];
+  }
+  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.2e-38f);
+
+  // ---- fragment addresses in a buffer ----
+  unsigned kfrag[KS], vfrag[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) kfrag[ks] = qcol * ROWB + (((2 * ks + half) ^ k_swizzle<CH>(qcol)) << 4);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    if constexpr (F32) {  // element 32 dt + qcol of rows 4 half + ...
+      const int row = 4 * half, d = 32 * dt + qcol;
+      vfrag[dt] = TILEB + row * ROWB + ((d / 4 ^ v_swizzle<CH, true>(row)) << 4) + d % 4 * 4;
+    } else {  // 8 bytes: elements 4 (i % 4) .. of row 4 half + i / 4, i = lane % 16
+      const int row = 4 * half + (lane & 15) / 4, d = 32 * dt + (lane & 16) + (lane & 3) * 4;
+      vfrag[dt] = TILEB + row * ROWB + ((d / 8 ^ v_swizzle<CH, false>(row)) << 4) + d % 8 * 2;
+    }
+  }
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  float m = -INFINITY, l = 0.f;  // m in units of the raw product
+
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, key0 = t * kPaKeys;
+    if (t + 1 < t1) {
+      issue_tile(t + 1, buf ^ 1);
+      if (t + 2 < t1) get_ids(t + 2);
+    }
+    if (key0 < w_hi && key0 + kPaKeys > w_lo) {
+      const lds_bytes base = (lds_bytes)smem + buf * 2 * TILEB;
+      // ---- scores: register r of s[kt] is key 32 kt + 8 (r / 4) + 4 half + r % 4 ----
+      f32x16 s[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const frag kf = *(const __attribute__((address_space(3))) frag*)(base + kfrag[ks] + kt * 32 * ROWB);
+          if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[ks][e], s[kt], 0, 0, 0);
+          } else {
+            s[kt] = PromptMma<T>::mul(kf, qf[ks], s[kt]);
+          }
+        }
+      }
+      if (key0 + kPaKeys > full_hi || key0 < full_lo || missing) {
+        unsigned long long there = ~0ull;
+        if (PAGED && missing) {
+          const int at = key0 + lane;
+          there = __ballot(at < w.keys && page_ok(lookup(min(at, w.keys - 1))));
+        }
+        there >>= 4 * half;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int k = 32 * kt + 8 * (r / 4) + r % 4, at = key0 + k + 4 * half;
+            if (at >= my_hi || at < my_lo || !(there >> k & 1)) s[kt][r] = -INFINITY;
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+      mx = xor32_max(mx);
+      // (m starts at -inf: the first finite maximum exceeds it by inf)
+      if (__ballot((mx - m) * c > 8.f || (m == -INFINITY && mx > m))) {
+        const float m_new = fmaxf(m, mx);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+        m = m_new;
+      }
+      const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mc));
+          sum += s[kt][r];
+        }
+        l += sum;
+        if constexpr (F32) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              const float vf = *(const __attribute__((address_space(3))) float*)(base + vfrag[dt] + (32 * kt + 8 * (r / 4) + r % 4) * ROWB);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[kt][r], o[dt], 0, 0, 0);
+            }
+        } else {
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          typedef short s16x8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            frag pf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pf[j] = (T)s[kt][8 * st + j];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              typedef __attribute__((address_space(3))) s16x4* tr_ptr;
+              const lds_bytes at = base + vfrag[dt] + (32 * kt + 16 * st) * ROWB;
+              const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+              const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 8 * ROWB));
+              const s16x8 both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+              o[dt] = PromptMma<T>::mul(__builtin_bit_cast(frag, both), pf, o[dt]);
+            }
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  if (wf0 >= pairs) return;
+
+  // ---- results: through the wave's part of LDS to whole rows ----
+  l = xor32_sum(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float odd = 0.f;  // NaN if any result is not finite
+  char* region = smem + wave * 32 * ROWB;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      typedef T vec __attribute__((ext_vector_type(4)));
+      vec y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = o[dt][4 * q + e] * inv;
+        odd = fmaf(x, 0.f, odd);
+        y[e] = (T)x;
+      }
+      const int byte = (32 * dt + 8 * q + 4 * half) * (int)sizeof(T);
+      *reinterpret_cast<vec*>(region + qcol * ROWB + ((byte >> 4 ^ k_swizzle<CH>(qcol)) << 4) + (byte & 15)) = y;
+    }
+  unsigned long long redo = __ballot(odd != 0.f);
+  const unsigned redo_rows = (unsigned)(redo | redo >> 32);
+  // (a wave's LDS instructions are served in order: it reads what its own lanes wrote)
+#pragma unroll
+  for (int j = 0; j < 32 / RPP; ++j) {
+    const int r = j * RPP + lane / CH, p = lane % CH;
+    const u32x4 y = *reinterpret_cast<const u32x4*>(region + r * ROWB + ((p ^ k_swizzle<CH>(r)) << 4));
+    const int f = wf0 + r;
+    if (f < pairs && !(redo_rows >> r & 1)) {
+      const int row = a.mul_div.page(f);
+      char* dst = a.out + ((w.q0 + row) * a.out_stride + (kvh * a.kv_mul + f - row * a.kv_mul) * HS) * (int64_t)sizeof(T) + 16 * p;
+      *KX_CKN(a, PP_OUT, reinterpret_cast<u32x4*>(dst), 16) = y;
+    }
+  }
+  // A pair whose result is not finite is computed again from the rows that it sees and no others: a NaN or an infinity in a
+  // V row that is hidden from it has met a weight of zero above.  Lanes take a key each for the scores, then a
+  // part of the row each for the sum.
+  for (unsigned left = redo_rows; left; left &= left - 1) {
+    const int f = wf0 + __builtin_ctz(left);
+    if (f >= pairs) break;
+    const int row = a.mul_div.page(f), head = kvh * a.kv_mul + f - row * a.kv_mul;
+    const int r_hi = hi_of(row), r_lo = lo_of(row);
+    auto key_row = [&](const T* base, int64_t stride, int t, bool& there) -> const T* {
+      if constexpr (PAGED) {
+        const int page = lookup(t);
+        there = page_ok(page);
+        return paged_row(base, page, t);
+      } else {
+        there = true;
+        return base + t * stride;
+      }
+    };
+    const T* qr = reinterpret_cast<const T*>(a.q) + (w.q0 + row) * a.q_stride + head * HS;
+    constexpr int VE = HS >= 64 ? HS / 64 : 1;
+    float rm = -INFINITY, rl = 0.f, acc[VE] = {};
+    const int d0 = min(lane * VE, HS - VE);
+    for (int base = r_lo; base < r_hi; base += 64) {
+      const int t = min(base + lane, r_hi - 1);
+      bool there;
+      const T* kr = key_row(kbase, k_stride, t, there);
+      float x = 0.f;
+      for (int d = 0; d < HS; d += 4) {
+        float k4[4], q4[4];
+        load4(KX_CKN(a, PP_K, kr + d, 4 * sizeof(T)), k4);
+        load4(KX_CKN(a, PP_Q, qr + d, 4 * sizeof(T)), q4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = fmaf(k4[e], a.scale < 0.f ? -q4[e] : q4[e], x);
+      }
+      if (!there || base + lane >= r_hi) x = -INFINITY;
+      const unsigned long long seen = __ballot(there && base + lane < r_hi);
+      const float nm = fmaxf(rm, wave_max(x));
+      const float alpha = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((rm - nm) * c);
+      const float p = __builtin_amdgcn_exp2f((x - (nm == -INFINITY ? 0.f : nm)) * c);
+      rm = nm;
+      rl = rl * alpha + wave_sum(p);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] *= alpha;
+      for (int j = 0; j < 64 && base + j < r_hi; ++j) {
+        const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
+        if (!(seen >> j & 1)) continue;
+        bool ok;
+        const T* vr = key_row(vbase, v_stride, base + j, ok) + d0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] = fmaf(pj, (float)*KX_CK(a, PP_V, vr + e), acc[e]);
+      }
+    }
+    if (lane * VE < HS) {
+      T* dst = reinterpret_cast<T*>(a.out) + (w.q0 + row) * a.out_stride + head * HS + d0;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) *KX_CK(a, PP_OUT, dst + e) = (T)(rl == 0.f ? 0.f : acc[e] / rl);
+    }
+  }
+}
+
+template <typename T, int HS, int MODE, int NW>
+static int prompt_launch(const PromptArgs& a, hipStream_t s) {
+  constexpr int lds = 2 * 2 * kPaKeys * HS * (int)sizeof(T);
+  static OncePerDevice limit;
+  if (lds > 32768)
+    if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, NW>), lds)) return rc;
+  // blocks of the sequences: an even share of all pairs and one more each
+  const int64_t items = (int64_t)a.q_rows * a.kv_mul / (NW * 32) + a.batch;
+  if (items * a.kv_heads > 0x7fffffffll) return KX_ELIMIT;
+  hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, NW>), dim3((unsigned)(items * a.kv_heads)), dim3(NW * 64), lds, s, a);
+  KX_LAUNCH_CHECK();
+  return KX_OK;
+}
+template <typename T, int HS>
+static int prompt_mode(const PromptArgs& a, hipStream_t s) {
+  if (!a.kv.table) return prompt_launch<T, HS, PA_PACKED, 8>(a, s);
+  if (a.kv.div.size % 16 == 0) return prompt_launch<T, HS, PA_BLOCK_PAGES, 8>(a, s);
+  return prompt_launch<T, HS, PA_ANY_PAGES, 8>(a, s);
+}
+template <typename T>
+static int prompt_hs(const PromptArgs& a, int hs, hipStream_t s) {
+  return hs == 32 ? prompt_mode<T, 32>(a, s) : hs == 64 ? prompt_mode<T, 64>(a, s) : prompt_mode<T, 128>(a, s);
 }
 
 }  // namespace kx
@@ -63,7 +501,7 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
   if (!head_size_known(d->head_size)) return KX_EUNSUPPORTED;
   if (d->window < 0 || (d->window > 0 && !d->causal)) return KX_EINVAL;
   const int64_t q_dim = (int64_t)d->head_num * d->head_size, kv_dim = (int64_t)d->kv_head_num * d->head_size;
-  const size_t unit = 16 / kind_bytes(d->type);
+  const size_t bytes = kind_bytes(d->type), unit = 16 / bytes;
   if (!d->q || !d->out || !d->cu_q || (uintptr_t)d->cu_q % 4 || !aligned16(d->q) || !aligned16(d->out) ||
       !stride_ok(d->q_stride, q_dim, unit) || !stride_ok(d->out_stride, q_dim, unit))
     return KX_EINVAL;
@@ -75,20 +513,28 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
     if (d->pages->kv_head_num != d->kv_head_num || d->pages->head_size != d->head_size || d->pages->batch != d->batch)
       return KX_EINVAL;
     a.kv = paged_view(*d->pages);
+    a.k = a.kv.key;
+    a.v = a.kv.value;
   } else {
     if (!d->k || !d->v || !d->cu_k || (uintptr_t)d->cu_k % 4 || d->k_rows < 0 || !aligned16(d->k) || !aligned16(d->v) ||
         !stride_ok(d->k_stride, kv_dim, unit) || !stride_ok(d->v_stride, kv_dim, unit))
       return KX_EINVAL;
+    // a tile's rows are addressed by 31-bit offsets from its first one
+    if ((uint64_t)d->k_stride * bytes * kPaKeys > 0x7fffffffull || (uint64_t)d->v_stride * bytes * kPaKeys > 0x7fffffffull)
+      return KX_EUNSUPPORTED;
+    a.k = static_cast<const char*>(d->k);
+    a.v = static_cast<const char*>(d->v);
   }
-  a.q = d->q; a.k = d->k; a.v = d->v; a.out = d->out; a.cu_q = d->cu_q; a.cu_k = d->cu_k;
+  const int32_t kv_mul = d->head_num / d->kv_head_num;
+  if ((int64_t)d->q_rows * kv_mul > 0x7fff0000ll) return KX_ELIMIT;  // (row, head) pairs are counted in 31 bits
+  a.q = static_cast<const char*>(d->q); a.out = static_cast<char*>(d->out); a.cu_q = d->cu_q; a.cu_k = d->cu_k;
   a.q_stride = d->q_stride; a.k_stride = d->k_stride; a.v_stride = d->v_stride; a.out_stride = d->out_stride;
-  a.batch = d->batch; a.head_num = d->head_num; a.kv_heads = d->kv_head_num; a.head_size = d->head_size;
+  a.batch = d->batch; a.kv_heads = d->kv_head_num; a.kv_mul = kv_mul; a.mul_div = page_div(kv_mul);
   a.q_rows = d->q_rows; a.k_rows = d->k_rows; a.causal = d->causal; a.window = d->window; a.scale = d->scale;
-  const dim3 grid(d->head_num, d->q_rows), block(256);
+  const void* operands[] = {a.q, a.k, a.v, a.out, a.cu_q, a.cu_k, a.kv.table, a.kv.seq_lens};
+  for (int i = 0; i < 8; ++i) KX_BSET(a, i, operands[i]);
+  (void)operands;
   hipStream_t s = (hipStream_t)stream;
-  if (d->type == KX_F16) hipLaunchKernelGGL(prompt_attn_simple_kernel<_Float16>, grid, block, 0, s, a);
-  else if (d->type == KX_BF16) hipLaunchKernelGGL(prompt_attn_simple_kernel<__bf16>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(prompt_attn_simple_kernel<float>, grid, block, 0, s, a);
-  KX_LAUNCH_CHECK();
-  return KX_OK;
+  return d->type == KX_F16 ? prompt_hs<_Float16>(a, d->head_size, s)
+         : d->type == KX_BF16 ? prompt_hs<__bf16>(a, d->head_size, s) : prompt_hs<float>(a, d->head_size, s);
 }
