@@ -1,10 +1,38 @@
-// Log probabilities of given tokens, entropy and the best alternatives of rows of logits.
+// Log probabilities of given tokens, entropy and the best alternatives of rows of logits, in one pass over them.
+//
+//   m = a reference near max x,  z = sum e^{x - m},  s = sum (x - m) e^{x - m}
+//   log p_t = (x_t - m) - ln z,   entropy = ln z - s / z
+//
+// Bound: the row is read once (rows * vocab * element size); about ten vector instructions per element, four of them the
+// exponential, are three quarters of that time for 16-bit logits.
+//
+// Split: a workgroup takes a row, or with few rows one of up to 64 parts of it; the parts' sums and lists meet in the
+// workspace and the workgroup that arrives last joins them in their order.
+//
+// Alternatives without a second pass: a lane keeps its largest value of all and of each of eight groups of its loads.  The
+// top_n-th largest of a wave's 64 lane maxima is at most the top_n-th largest value, so only the few groups that
+// reach it are read again (they are in the caches), and their elements at or above it (some tens) are ranked by counting.
+// Where more of them are alike than the list holds, the part is gone through in order of index instead.
+//
+// The reference m is shared by a wave and follows a new maximum only when that lies more than 16 above it (e^16 is far
+// from the range of fp32), so the sums are hardly ever rescaled.
 #include <math.h>
 
 #define KX_FILE_ID 13
 #include "paged.hpp"
 
 namespace kx {
+
+enum LogprobsOperand { PL_X, PL_TOKENS, PL_LOGPROB, PL_ENTROPY, PL_IDS, PL_TOP, PL_WS };
+
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
+constexpr int kLpUnroll = 4;      // vectors of 16 bytes in flight per lane
+constexpr int kLpGroups = 8;      // groups of a lane's loads
+constexpr int kLpList = 512;      // elements that are ranked at once
+constexpr int kLpMaxParts = 64;   // one lane each in the join
+constexpr int kLpSlots = 1024;    // workgroups that few rows are cut for
+constexpr int kLpRecord = 16 + 8 * KX_LOGPROBS_TOP_MAX;  // bytes: m, z, s, -, then the list
+constexpr size_t kLpTicketBytes = (size_t)kLpSlots * 64;
 
 struct LogprobsArgs {
   const void* logits;
@@ -13,91 +41,338 @@ struct LogprobsArgs {
   float* entropy;
   int32_t* top_ids;
   float* top_logprobs;
+  char* records;      // [row][part]
+  unsigned* tickets;  // [row], 64 bytes apart
   int64_t row_stride;
-  int32_t rows, vocab, top_n;
+  int32_t rows, vocab, top_n, parts;
+  KX_BFIELD(7)
 };
 
-// Order of the alternatives as an unsigned whole number: larger value first, the lower index ahead among equal
-// ones, NaN below -inf.
-__device__ __forceinline__ unsigned long long rank_of(float x, int index) {
+// Order of the alternatives as an unsigned whole number: larger value first, the lower index ahead among equal ones
+// (both zeros are equal), NaN below -inf.  No element has key 0.
+__device__ __forceinline__ unsigned long long key_of(float x, int index) {
   unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
-  u = u >> 31 ? ~u : u | 0x80000000u;  // monotone in x
+  u = u >> 31 ? ~u : u | 0x80000000u;
   if (x != x) u = 0u;
   return (unsigned long long)u << 32 | (0xffffffffu - (unsigned)index);
 }
+__device__ __forceinline__ float value_of_key(unsigned long long k) {
+  const unsigned u = (unsigned)(k >> 32);
+  return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ int index_of_key(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
 
-__device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v) {
-  for (int off = 32; off; off >>= 1) {
-    const unsigned long long o = __shfl_xor(v, off);
-    v = o > v ? o : v;
+__device__ __forceinline__ unsigned umax_dpp_row(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+  v = umax_dpp_row(v);
+  unsigned a = v, b = v;
+  permlane16_swap(a, b);
+  v = max(a, b);
+  a = v, b = v;
+  permlane32_swap(a, b);
+  return max(a, b);
+}
+
+template <typename T> struct LogitVec;  // 16 bytes of logits
+template <> struct LogitVec<float> {
+  static constexpr int N = 4;
+  static constexpr unsigned kNone = 0xff800000u;  // -inf
+  static __device__ __forceinline__ float get(const u32x4& v, int i) { return __uint_as_float(v[i]); }
+};
+template <> struct LogitVec<_Float16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kNone = 0xfc00fc00u;
+  static __device__ __forceinline__ float get(const u32x4& v, int i) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(v[i / 2] >> (i % 2 * 16)));
   }
-  return v;
+};
+template <> struct LogitVec<__bf16> {
+  static constexpr int N = 8;
+  static constexpr unsigned kNone = 0xff80ff80u;
+  static __device__ __forceinline__ float get(const u32x4& v, int i) {
+    return __uint_as_float(i % 2 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+  }
+};
+
+// sums relative to m
+struct LogSums {
+  float m, z, s;
+};
+// The same sums relative to a larger reference.  m = -inf: nothing but -inf so far (z = 0) or nothing but NaN.
+__device__ __forceinline__ void rebase(LogSums& a, float m) {
+  if (a.m != -INFINITY) {
+    const float d = a.m - m, f = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+    a.s = d > -150.f ? (a.s + a.z * d) * f : a.s * 0.f;
+    a.z *= f;
+  }
+  a.m = m;
+}
+
+// The top_n largest of the `count` keys in LDS, in falling order: a key's place is the number of keys above it.
+__device__ __forceinline__ void rank_keys(const unsigned long long* keys, int count, int top_n, unsigned long long* out) {
+  for (int i = threadIdx.x; i < count; i += kLpThreads) {
+    const unsigned long long mine = keys[i];
+    int above = 0;
+    for (int j = 0; j < count; ++j) above += keys[j] > mine;
+    if (above < top_n) out[above] = mine;
+  }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void logprobs_simple_kernel(const LogprobsArgs a) {
-  __shared__ float red[4], red2[4];
-  __shared__ unsigned long long best[4];
-  const int row = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsArgs a) {
+  typedef LogitVec<T> Vec;
+  constexpr int N = Vec::N;
+  // group maxima and the list; in the join the parts' lists
+  __shared__ __attribute__((aligned(16))) unsigned long long sm_raw[kLpMaxParts * KX_LOGPROBS_TOP_MAX];
+  static_assert(sizeof(sm_raw) >= kLpGroups * kLpThreads * 4 + kLpList * 8, "");
+  float* sm_group = reinterpret_cast<float*>(sm_raw);
+  unsigned long long* sm_list = sm_raw + kLpGroups * kLpThreads / 2;
+  __shared__ unsigned long long sm_top[KX_LOGPROBS_TOP_MAX];
+  __shared__ float sm_sums[kLpWaves][3], sm_least[kLpWaves];
+  __shared__ int sm_count, sm_last;
+
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  float m = -INFINITY;
-  bool odd = false;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float v = (float)x[i];
-    odd |= v != v || v == INFINITY;
-    m = fmaxf(m, v);
+  // the row from its first 16-byte boundary on in vectors; the elements ahead and behind belong to the outer parts
+  const int ahead = min(a.vocab, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)));
+  const int vectors = (a.vocab - ahead) / N, behind0 = ahead + vectors * N;
+  const int v0 = (int)((int64_t)vectors * part / a.parts), v1 = (int)((int64_t)vectors * (part + 1) / a.parts);
+  const u32x4* xv = reinterpret_cast<const u32x4*>(x + ahead);
+  int extra = -1;  // this thread's element ahead or behind
+  if (part == 0 && tid < ahead) extra = tid;
+  if (part == a.parts - 1 && tid >= 8 && behind0 + tid - 8 < a.vocab) extra = behind0 + tid - 8;
+  const float xe = extra >= 0 ? (float)*KX_CK(a, PL_X, x + extra) : -INFINITY;
+
+  if (tid == 0) sm_count = 0;
+  LogSums sums = {wave_max(xe), 0.f, 0.f};
+  float largest = fmaxf(xe, -INFINITY);  // (no NaN)
+  if (extra >= 0) {
+    const float d = xe - (sums.m == -INFINITY ? 0.f : sums.m), e = __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
+    sums.z = e;
+    sums.s = fmaxf(d, -150.f) * e;
   }
-  odd = __syncthreads_or(odd);
-  m = wave_max(m);
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  odd |= m == -INFINITY;
-  __syncthreads();
-  float z = 0.f, s = 0.f;
-  for (int i = tid; i < a.vocab; i += 256) {
-    const float d = (float)x[i] - m, e = expf(d);
-    z += e;
-    if (e > 0.f) s = fmaf(d, e, s);
-  }
-  z = wave_sum(z);
-  s = wave_sum(s);
-  if ((tid & 63) == 0) red[tid >> 6] = z, red2[tid >> 6] = s;
-  __syncthreads();
-  z = (red[0] + red[1]) + (red[2] + red[3]);
-  s = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-  const float lz = odd ? NAN : logf(z);
-  if (tid == 0) {
-    if (a.logprob) {
-      const int t = a.tokens[row];
-      a.logprob[row] = t < 0 ? 0.f : t >= a.vocab ? NAN : ((float)x[t] - m) - lz;
+  const int per_step = kLpThreads * kLpUnroll;
+  const int steps = (v1 - v0 + per_step - 1) / per_step, group_steps = (steps + kLpGroups - 1) / kLpGroups;
+  auto load_step = [&](int step, u32x4 (&v)[kLpUnroll]) {
+    const int at = v0 + step * per_step + tid;
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) {
+      const int i = at + u * kLpThreads;
+      v[u] = *KX_CK(a, PL_X, xv + min(i, v1 - 1));
     }
-    if (a.entropy) a.entropy[row] = lz - s / z;
-  }
-  unsigned long long below = ~0ull;
-  for (int n = 0; n < a.top_n; ++n) {
-    unsigned long long b = 0;
-    for (int i = tid; i < a.vocab; i += 256) {
-      const unsigned long long r = rank_of((float)x[i], i);
-      if (r < below && r > b) b = r;
+    if (step == steps - 1) {
+#pragma unroll
+      for (int u = 0; u < kLpUnroll; ++u)
+        if (at + u * kLpThreads >= v1) v[u] = u32x4{Vec::kNone, Vec::kNone, Vec::kNone, Vec::kNone};
     }
-    b = wave_max_u64(b);
+  };
+  int step = 0;
+  for (int group = 0; step < steps; ++group) {
+    float group_max = -INFINITY;
+    const int end = min(step + group_steps, steps);
+    for (; step < end; ++step) {
+      u32x4 v[kLpUnroll];
+      load_step(step, v);
+      float mx = Vec::get(v[0], 0);
+#pragma unroll
+      for (int u = 0; u < kLpUnroll; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) mx = fmaxf(mx, Vec::get(v[u], i));
+      mx = fmaxf(mx, -INFINITY);  // (a first element that is NaN)
+      group_max = fmaxf(group_max, mx);
+      if (__ballot(mx > sums.m + 16.f)) rebase(sums, fmaxf(sums.m, wave_max(mx)));
+      const float m = sums.m == -INFINITY ? 0.f : sums.m;
+      float z0 = 0.f, z1 = 0.f, s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int u = 0; u < kLpUnroll; ++u)
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const float d0 = Vec::get(v[u], i) - m, d1 = Vec::get(v[u], i + 1) - m;
+          const float e0 = __builtin_amdgcn_exp2f(d0 * 1.4426950408889634f), e1 = __builtin_amdgcn_exp2f(d1 * 1.4426950408889634f);
+          z0 += e0;
+          z1 += e1;
+          s0 = fmaf(fmaxf(d0, -150.f), e0, s0);  // (-inf adds nothing: e is zero)
+          s1 = fmaf(fmaxf(d1, -150.f), e1, s1);
+        }
+      sums.z += z0 + z1;
+      sums.s += s0 + s1;
+    }
+    sm_group[group * kLpThreads + tid] = group_max;
+    largest = fmaxf(largest, group_max);
+  }
+  sums.z = wave_sum(sums.z);
+  sums.s = wave_sum(sums.s);
+  if (lane == 0) {
+    sm_sums[wave][0] = sums.m;
+    sm_sums[wave][1] = sums.z;
+    sm_sums[wave][2] = sums.s;
+  }
+  if (a.top_n > 0) {
+    // the top_n-th largest of the lanes' maxima, the lower lane ahead among equal ones
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < 64; ++j) {
+      const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(largest), j));
+      above += other > largest || (other == largest && j < lane);
+    }
+    const unsigned long long at = __ballot(above == a.top_n - 1);
+    if (lane == 0) sm_least[wave] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(largest), __builtin_ctzll(at)));
+  }
+  __syncthreads();
+  LogSums all = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w) all.m = fmaxf(all.m, sm_sums[w][0]);
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w) {
+    LogSums one = {sm_sums[w][0], sm_sums[w][1], sm_sums[w][2]};
+    rebase(one, all.m);
+    all.z += one.z;
+    all.s += one.s;
+  }
+
+  if (a.top_n > 0) {
+    float least = sm_least[0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; ++w) least = fmaxf(least, sm_least[w]);
+    auto take = [&](float v, int index) {
+      if (v < least) return;  // (NaN stays: it may be among the best of a row with less than top_n others)
+      const int at = atomicAdd(&sm_count, 1);
+      if (at < kLpList) sm_list[at] = key_of(v, index);
+    };
+    if (extra >= 0) take(xe, extra);
+    for (int group = 0; group * group_steps < steps; ++group) {
+      if (sm_group[group * kLpThreads + tid] < least) continue;
+      for (int st = group * group_steps; st < min((group + 1) * group_steps, steps); ++st) {
+        u32x4 v[kLpUnroll];
+        load_step(st, v);
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+          const int i = v0 + st * per_step + u * kLpThreads + tid;
+          if (i < v1) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) take(Vec::get(v[u], e), ahead + i * N + e);
+          }
+        }
+      }
+    }
     __syncthreads();
-    if ((tid & 63) == 0) best[tid >> 6] = b;
+    int count = sm_count;
+    if (tid < KX_LOGPROBS_TOP_MAX) sm_top[tid] = 0;
     __syncthreads();
-    for (int w = 0; w < 4; ++w) b = best[w] > b ? best[w] : b;
-    below = b;
+    if (count > kLpList) {
+      // too many alike: in order of index, 256 at a time, the best so far kept at the head of the list
+      const int e0 = part == 0 ? 0 : ahead + v0 * N, e1 = part == a.parts - 1 ? a.vocab : ahead + v1 * N;
+      unsigned long long least_key = 0;
+      if (tid == 0) sm_count = 0;
+      __syncthreads();
+      for (int base = e0; base < e1; base += kLpThreads) {
+        const int i = base + tid;
+        const unsigned long long key = i < e1 ? key_of((float)*KX_CK(a, PL_X, x + i), i) : 0;
+        if (key > least_key) sm_list[atomicAdd(&sm_count, 1)] = key;  // at most kLpList: see below
+        __syncthreads();
+        count = sm_count;
+        __syncthreads();
+        if (count > kLpList - kLpThreads) {
+          rank_keys(sm_list, count, a.top_n, sm_top);
+          __syncthreads();
+          if (tid < a.top_n) sm_list[tid] = sm_top[tid];
+          least_key = sm_top[a.top_n - 1];
+          if (tid == 0) sm_count = a.top_n;
+          __syncthreads();
+        }
+      }
+      count = sm_count;
+    }
+    rank_keys(sm_list, count, a.top_n, sm_top);
+    __syncthreads();
+  }
+
+  unsigned long long best = tid < a.top_n ? sm_top[tid] : 0;  // threads 0 .. top_n - 1 of the first wave
+  if (a.parts > 1) {
+    char* mine = a.records + (int64_t)(row * a.parts) * kLpRecord;
+    const __amdgpu_buffer_rsrc_t rec = __builtin_amdgcn_make_buffer_rsrc(mine, 0, 0x7fffffff, 0x00020000);
+    // device-scope stores, acknowledged ahead of the ticket; device-scope loads behind it (no cache write-back)
+    KX_TOUCH(a, PL_WS, mine + part * kLpRecord, kLpRecord);
     if (tid == 0) {
-      const int i = (int)(0xffffffffu - (unsigned)b);
-      a.top_ids[(size_t)row * a.top_n + n] = i;
-      a.top_logprobs[(size_t)row * a.top_n + n] = ((float)x[i] - m) - lz;
+      const u32x4 s = {__float_as_uint(all.m), __float_as_uint(all.z), __float_as_uint(all.s), 0u};
+      __builtin_amdgcn_raw_buffer_store_b128(s, rec, part * kLpRecord, 0, 16);
+    }
+    if (tid < a.top_n)
+      __builtin_amdgcn_raw_buffer_store_b64(u32x2{(unsigned)best, (unsigned)(best >> 32)}, rec, part * kLpRecord + 16 + 8 * tid, 0, 16);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      sm_last = atomicInc(KX_CK(a, PL_WS, a.tickets + row * 16), (unsigned)a.parts - 1u) == (unsigned)a.parts - 1u;  // wraps to 0
+    }
+    __syncthreads();
+    if (!sm_last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int i = tid; i < a.parts * a.top_n; i += kLpThreads) {
+      const int p = i / a.top_n;
+      const u32x2 k = __builtin_amdgcn_raw_buffer_load_b64(rec, p * kLpRecord + 16 + 8 * (i - p * a.top_n), 0, 16);
+      sm_raw[i] = (unsigned long long)k.y << 32 | k.x;
+    }
+    const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(rec, min(lane, a.parts - 1) * kLpRecord, 0, 16);
+    LogSums one = {__uint_as_float(s.x), __uint_as_float(s.y), __uint_as_float(s.z)};
+    if (lane >= a.parts) one = LogSums{-INFINITY, 0.f, 0.f};
+    const float m = wave_max(one.m);
+    rebase(one, m);
+    all = LogSums{m, wave_sum(one.z), wave_sum(one.s)};
+    __syncthreads();
+    if (wave != 0) return;
+    // the parts' lists fall: take the largest head top_n times, lane p at part p's list
+    int at = 0;
+    unsigned long long head = lane < a.parts && a.top_n > 0 ? sm_raw[lane * a.top_n] : 0;
+    for (int n = 0; n < a.top_n; ++n) {
+      const unsigned hi = wave_umax((unsigned)(head >> 32));
+      const unsigned lo = wave_umax((unsigned)(head >> 32) == hi ? (unsigned)head : 0u);
+      const unsigned long long top = (unsigned long long)hi << 32 | lo;
+      if (lane == n) best = top;
+      if (head == top) {
+        ++at;
+        head = at < a.top_n ? sm_raw[lane * a.top_n + at] : 0;
+      }
     }
   }
+  if (wave != 0) return;
+  const bool odd = !(all.z > 0.f && all.z < INFINITY);
+  const float lz = odd ? NAN : logf(all.z);
+  if (lane == 0) {
+    if (a.logprob) {
+      const int t = *KX_CK(a, PL_TOKENS, a.tokens + row);
+      *KX_CK(a, PL_LOGPROB, a.logprob + row) =
+          t < 0 ? 0.f : t >= a.vocab ? NAN : ((float)*KX_CK(a, PL_X, x + t) - all.m) - lz;
+    }
+    if (a.entropy) *KX_CK(a, PL_ENTROPY, a.entropy + row) = lz - all.s / all.z;
+  }
+  if (lane < a.top_n) {
+    *KX_CK(a, PL_IDS, a.top_ids + ((int64_t)row * a.top_n + lane)) = index_of_key(best);
+    *KX_CK(a, PL_TOP, a.top_logprobs + ((int64_t)row * a.top_n + lane)) = (value_of_key(best) - all.m) - lz;
+  }
+}
+
+// Parts of a row: enough to fill the chip, each of two vectors per thread at least.
+static int logprobs_parts(int rows, int vocab, int kind) {
+  const int64_t least = (int64_t)kLpThreads * 2 * 16 / (int64_t)kind_bytes(kind);
+  int64_t parts = kLpSlots / rows;
+  if (parts > vocab / least) parts = vocab / least;
+  return parts < 1 ? 1 : parts > kLpMaxParts ? kLpMaxParts : (int)parts;
 }
 
 }  // namespace kx
 
-extern "C" size_t kx_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_n) { return rows <= 0 || vocab <= 0 || top_n < 0 ? 0 : 256; }
+extern "C" size_t kx_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_n) {
+  using namespace kx;
+  if (rows <= 0 || vocab <= 0 || top_n < 0) return 0;
+  return kLpTicketBytes + (size_t)kLpSlots * kLpRecord;  // the tickets' place is the same for every call
+}
 
 extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
   using namespace kx;
@@ -110,11 +385,28 @@ extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
   if (d->top_n > 0 && (!d->top_ids || !d->top_logprobs)) return KX_EINVAL;
   if (!d->workspace || d->workspace_bytes < kx_token_logprobs_workspace_bytes(d->rows, d->vocab, d->top_n)) return KX_EWORKSPACE;
   if ((uintptr_t)d->workspace % 256) return KX_EINVAL;
-  LogprobsArgs a{d->logits, d->tokens, d->logprob, d->entropy, d->top_ids, d->top_logprobs, d->row_stride, d->rows, d->vocab, d->top_n};
+  LogprobsArgs a{};
+  a.logits = d->logits;
+  a.tokens = d->tokens;
+  a.logprob = d->logprob;
+  a.entropy = d->entropy;
+  a.top_ids = d->top_ids;
+  a.top_logprobs = d->top_logprobs;
+  a.tickets = static_cast<unsigned*>(d->workspace);
+  a.records = static_cast<char*>(d->workspace) + kLpTicketBytes;
+  a.row_stride = d->row_stride;
+  a.rows = d->rows;
+  a.vocab = d->vocab;
+  a.top_n = d->top_n;
+  a.parts = logprobs_parts(d->rows, d->vocab, d->type);
+  const void* operands[] = {a.logits, a.tokens, a.logprob, a.entropy, a.top_ids, a.top_logprobs, d->workspace};
+  for (int i = 0; i < 7; ++i) KX_BSET(a, i, operands[i]);
+  (void)operands;
+  const dim3 grid((unsigned)a.rows * (unsigned)a.parts), block(kLpThreads);
   hipStream_t s = (hipStream_t)stream;
-  if (d->type == KX_F16) hipLaunchKernelGGL(logprobs_simple_kernel<_Float16>, dim3(d->rows), dim3(256), 0, s, a);
-  else if (d->type == KX_BF16) hipLaunchKernelGGL(logprobs_simple_kernel<__bf16>, dim3(d->rows), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(logprobs_simple_kernel<float>, dim3(d->rows), dim3(256), 0, s, a);
+  if (d->type == KX_F16) hipLaunchKernelGGL(logprobs_kernel<_Float16>, grid, block, 0, s, a);
+  else if (d->type == KX_BF16) hipLaunchKernelGGL(logprobs_kernel<__bf16>, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(logprobs_kernel<float>, grid, block, 0, s, a);
   KX_LAUNCH_CHECK();
   return KX_OK;
 }
