@@ -17,6 +17,11 @@
 // value per lane and the weights are already the B operand of O^T = V^T P^T; the A operand V^T comes out of row-major V by
 // transposing LDS reads (16-bit types), or one element per lane (fp32).
 //
+// Reached: 1.0 PFLOP/s on a prompt of 4096 (32 heads over 8, 128 wide, bf16: 134 us), at 2.0 GHz: the chip's power, which holds
+// a library product of 8192 x 8192 x 8192 to 1.09 PFLOP/s as well.  Half the cycles are matrix instructions and half vector
+// ones there.  Tried and no faster: the two waves of a SIMD half a step apart (150 us), the next scores and the last
+// second product between a wave's vector instructions (143, with spills), waiting later for the LDS-DMA (the same).
+//
 // Rounding: products of 16-bit operands are exact in fp32 and summed there, softmax in fp32, weights rounded to the
 // type for the second product, the sum of the weights unrounded.  The running maximum follows only when it is
 // exceeded by more than 2^8: weights up to 256 have the same relative precision, and the rescaling pass is rare.
@@ -31,7 +36,9 @@ namespace kx {
 
 enum PromptOperand { PP_Q, PP_K, PP_V, PP_OUT, PP_CUQ, PP_CUK, PP_TABLE, PP_LENS };
 
-constexpr int kPaKeys = 64;  // keys per tile
+constexpr int kPaWaves = 8;  // waves of a workgroup
+// keys per tile: as many as let two buffers of a tile per group of waves fit LDS
+template <typename T> __host__ __device__ constexpr int pa_keys() { return sizeof(T) == 4 ? 32 : 64; }
 
 enum { PA_PACKED = 0, PA_BLOCK_PAGES = 1, PA_ANY_PAGES = 2 };  // where rows are: see row sources below
 
@@ -64,29 +71,44 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
   const int lane = lane_id();
   int done = 0;
   for (int base = 0; base < a.batch; base += 64) {
-    const int b = base + lane;
-    int q0 = 0, n = 0;
+    int b = base + lane, q0 = 0, n = 0, k0 = 0, keys = 0;
     if (b < a.batch) {
       q0 = clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b), a.q_rows);
       n = max(clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b + 1), a.q_rows) - q0, 0);
+      if (PAGED) {
+        keys = min(max(*KX_CK(a, PP_LENS, a.kv.seq_lens + b), 0), a.kv.capacity());
+      } else {
+        k0 = clamp_row(*KX_CK(a, PP_CUK, a.cu_k + b), a.k_rows);
+        keys = max(clamp_row(*KX_CK(a, PP_CUK, a.cu_k + b + 1), a.k_rows) - k0, 0);
+      }
+    }
+    // The sequences (64 at a time) in falling order of their keys, each one's last blocks first: long chains of tiles
+    // start early.  (Six pieces of 118 .. 1024 rows over 425 .. 4298 keys: 178 us in index order, 146 so, one group.)
+    if (a.batch > 1) {
+      int place = 0;
+      for (int j = 0; j < min(a.batch - base, 64); ++j) {
+        const int other = __builtin_amdgcn_readlane(keys, j);
+        place += other > keys || (other == keys && j < lane);
+      }
+      if (b >= a.batch) place = lane;
+      const int from = __builtin_amdgcn_ds_permute(place << 2, lane) << 2;
+      b = base + (from >> 2);
+      q0 = __builtin_amdgcn_ds_bpermute(from, q0);
+      n = __builtin_amdgcn_ds_bpermute(from, n);
+      k0 = __builtin_amdgcn_ds_bpermute(from, k0);
+      keys = __builtin_amdgcn_ds_bpermute(from, keys);
     }
     const int blocks = (int)(((int64_t)n * a.kv_mul + ROWS - 1) / ROWS);
     const int upto = wave_scan(blocks);
     const unsigned long long past = __ballot(done + upto > item);
     if (past) {
       const int l = __builtin_ctzll(past);
-      w.b = base + l;
+      w.b = __builtin_amdgcn_readlane(b, l);
       w.q0 = __builtin_amdgcn_readlane(q0, l);
       w.n = __builtin_amdgcn_readlane(n, l);
-      // a sequence's last blocks first: they see the most keys
+      w.k0 = __builtin_amdgcn_readlane(k0, l);
+      w.keys = __builtin_amdgcn_readlane(keys, l);
       w.block = done + __builtin_amdgcn_readlane(upto, l) - 1 - item;
-      if (PAGED) {
-        w.k0 = 0;
-        w.keys = min(max(*KX_CK(a, PP_LENS, a.kv.seq_lens + w.b), 0), a.kv.capacity());
-      } else {
-        w.k0 = clamp_row(*KX_CK(a, PP_CUK, a.cu_k + w.b), a.k_rows);
-        w.keys = max(clamp_row(*KX_CK(a, PP_CUK, a.cu_k + w.b + 1), a.k_rows) - w.k0, 0);
-      }
       return true;
     }
     done += __builtin_amdgcn_readlane(upto, 63);
@@ -105,6 +127,15 @@ __device__ __forceinline__ int v_swizzle(int row) {
   return CH == 16 ? (row & 3) << 2 : CH == 8 ? (row >> 1 & 1) << 2 : 0;
 }
 
+// A transposing LDS read: of the 4 rows x 16 elements that 16 lanes point at (8 bytes each, row i / 4 for lane i), lane i
+// gets column i.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4* lds_tr_ptr;
+__device__ __forceinline__ s16x4 read_transposed(lds_tr_ptr p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
+
 template <typename T> struct PromptMma;
 template <> struct PromptMma<_Float16> {
   typedef f16x8 frag;
@@ -120,21 +151,26 @@ template <> struct PromptMma<__bf16> {
 };
 template <> struct PromptMma<float> { typedef f32x4 frag; };
 
-template <typename T, int HS, int MODE, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArgs a) {
+// KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
+// chains of tiles and more workgroups where there are few pairs.
+template <typename T, int HS, int MODE, int KG>
+__global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const PromptArgs a) {
+  constexpr int NW = kPaWaves, PW = NW / KG;     // waves, those of a group
+  constexpr int PAIRS = PW * 32;                 // pairs of the workgroup
+  constexpr int KT = pa_keys<T>();
   constexpr bool F32 = sizeof(T) == 4, PAGED = MODE != PA_PACKED;
   constexpr int ROWB = HS * (int)sizeof(T);      // bytes of a row
   constexpr int CH = ROWB / 16;                  // its pieces
   constexpr int RPP = 1024 / ROWB;               // rows per DMA instruction
-  constexpr int TILEB = kPaKeys * ROWB;          // K (or V) bytes of a tile
+  constexpr int TILEB = KT * ROWB;               // K (or V) bytes of a tile
   constexpr int KP = TILEB / 1024;               // DMA instructions for them
-  constexpr int PER = 2 * KP / NW;               // per wave
+  constexpr int PER = 2 * KP * KG / NW;          // per wave and buffer
   constexpr int DT = HS / 32;                    // output tiles
   // fp16 weights are held 2^7 times as large: at most 2^15, and whole down to 2^-21 of the largest
   constexpr float kShift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
   constexpr int KS = HS * (int)sizeof(T) / 32;   // 32-byte steps of the first product
-  static_assert(2 * KP % NW == 0, "");
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers: K tile, V tile
+  static_assert(2 * KP * KG % NW == 0, "");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers of KG tiles, K and V each
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef const __attribute__((address_space(3))) char* lds_bytes;
 
@@ -142,17 +178,18 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
   const int qcol = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.x % a.kv_heads;
   PromptWork w;
-  if (!find_prompt<NW * 32, PAGED>(a, blockIdx.x / a.kv_heads, w)) return;
+  if (!find_prompt<PAIRS, PAGED>(a, blockIdx.x / a.kv_heads, w)) return;
+  const int group = wave / PW;
 
   // ---- this workgroup's and this wave's pairs, and what they see ----
-  const int pairs = w.n * a.kv_mul, f0 = w.block * NW * 32;
+  const int pairs = w.n * a.kv_mul, f0 = w.block * PAIRS;
   const int p0 = w.keys - w.n;  // position of row 0, below zero with fewer keys than rows
   auto hi_of = [&](int row) { return a.causal ? max(min(p0 + row + 1, w.keys), 0) : w.keys; };
   auto lo_of = [&](int row) { return a.window > 0 ? max(p0 + row - a.window + 1, 0) : 0; };
   auto row_of = [&](int f) { return a.mul_div.page(min(f, pairs - 1)); };
-  const int hi = hi_of(row_of(f0 + NW * 32 - 1)), lo = min(lo_of(row_of(f0)), hi);
-  const int t0 = lo / kPaKeys, t1 = hi > lo ? (hi + kPaKeys - 1) / kPaKeys : t0;
-  const int wf0 = f0 + wave * 32;
+  const int hi = hi_of(row_of(f0 + PAIRS - 1)), lo = min(lo_of(row_of(f0)), hi);
+  const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
+  const int wf0 = f0 + wave % PW * 32;
   const int first_row = row_of(wf0), last_row = row_of(wf0 + 31);
   const int w_hi = wf0 < pairs ? hi_of(last_row) : 0, w_lo = lo_of(first_row);
   const int full_hi = hi_of(first_row), full_lo = lo_of(last_row);  // every pair of the wave sees these keys
@@ -169,60 +206,70 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
   auto paged_row = [&](const T* base, int page, int t) {
     return base + (page_ok(page) ? page : 0) * a.kv.page_stride + (t - a.kv.div.page(t) * a.kv.div.size) * a.kv.row_stride;
   };
-  // piece i of this wave: rows 16-byte pieces of K (q < KP) or V; a lane's row in the tile and its piece of the row
-  auto piece_row = [&](int i) { return (wave + NW * i) % KP * RPP + lane / CH; };
-  auto piece_is_k = [&](int i) { return wave + NW * i < KP; };
-  unsigned off[PER];  // byte offset of the lane's piece from the tile's first row (packed), or in its row (pages)
+  // The KG tiles of a buffer are consecutive, so its K rows are KG * KT consecutive keys.  DMA instruction q of a
+  // buffer: tile q / (2 KP), K rows then V rows; the first of its rows among the keys, and a lane's.
+  auto piece_first = [&](int i) { return (wave + NW * i) / (2 * KP) * KT + (wave + NW * i) % KP * RPP; };
+  auto piece_row = [&](int i) { return piece_first(i) + lane / CH; };
+  auto piece_is_k = [&](int i) { return (wave + NW * i) % (2 * KP) < KP; };
+  // a lane's byte offset from the first row of the buffer (packed), from the first row of the instruction's 16-row block,
+  // or within its row (pages)
+  unsigned off[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int row = piece_row(i);
-    const int c = lane % CH ^ (piece_is_k(i) ? k_swizzle<CH>(row) : v_swizzle<CH, F32>(row));
-    off[i] = 16u * c + (PAGED ? 0u : (unsigned)(row * (int)(piece_is_k(i) ? k_stride : v_stride) * (int)sizeof(T)));
+    const int row = piece_row(i), from = MODE == PA_PACKED ? row : MODE == PA_BLOCK_PAGES ? lane / CH : 0;
+    off[i] = 16u * (lane % CH ^ (piece_is_k(i) ? k_swizzle<CH>(row) : v_swizzle<CH, F32>(row))) +
+             (unsigned)(from * (int)(piece_is_k(i) ? k_stride : v_stride) * (int)sizeof(T));
   }
-  // pages of the next tile's pieces: one per piece where pages are whole 16-row blocks, else one per lane
+  // Pages of the next buffer's rows, requested a step ahead: one per instruction where pages are whole 16-row blocks, else
+  // one per lane.  (By vector loads in both cases: the end of a step waits for those anyway, while a scalar load would
+  // have the next fragment reads wait for it.)
   int ids[PAGED ? PER : 1];
   auto get_ids = [&](int t) {
     if constexpr (PAGED) {
+      int zero;
+      asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         if constexpr (MODE == PA_BLOCK_PAGES)
-          ids[i] = __builtin_amdgcn_readfirstlane(
-              lookup(min(t * kPaKeys + (wave + NW * i) % KP * RPP, (w.keys - 1) & ~(RPP - 1))));
+          ids[i] = lookup(min(t * KT + piece_first(i), (w.keys - 1) & ~(RPP - 1)) + zero);
         else
-          ids[i] = lookup(min(t * kPaKeys + piece_row(i), w.keys - 1));
+          ids[i] = lookup(min(t * KT + piece_row(i), w.keys - 1));
       }
     }
   };
   auto issue_tile = [&](int t, int buf) {
-    const int key0 = t * kPaKeys;
-    const bool whole = key0 + kPaKeys <= w.keys;
+    const int key0 = t * KT;
+    const bool whole = key0 + KG * KT <= w.keys;  // else rows behind the last are replaced by it
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const bool is_k = piece_is_k(i);
       const T* base = is_k ? kbase : vbase;
       const char* src;
-      if constexpr (PAGED) {
-        int key = key0 + piece_row(i);
-        if (!whole) {  // rows behind the last are replaced by it, within the page of its block
-          if (MODE == PA_BLOCK_PAGES) key = min(key0 + (wave + NW * i) % KP * RPP, (w.keys - 1) & ~(RPP - 1)) + lane / CH;
-          key = min(key, w.keys - 1);
-        }
-        src = reinterpret_cast<const char*>(paged_row(base, ids[i], key)) + off[i];
+      if constexpr (MODE == PA_ANY_PAGES) {
+        src = reinterpret_cast<const char*>(paged_row(base, ids[i], min(key0 + piece_row(i), w.keys - 1))) + off[i];
       } else {
         const int64_t stride = is_k ? k_stride : v_stride;
-        const char* tile = reinterpret_cast<const char*>(base + (int64_t)key0 * stride);
-        if (whole) src = tile + off[i];
-        else src = tile + off[i] - (int64_t)max(piece_row(i) - (w.keys - 1 - key0), 0) * stride * (int)sizeof(T);
+        int first = key0;  // uniform
+        const char* from;
+        if constexpr (MODE == PA_BLOCK_PAGES) {
+          first = min(key0 + piece_first(i), (w.keys - 1) & ~(RPP - 1));
+          from = reinterpret_cast<const char*>(paged_row(base, __builtin_amdgcn_readfirstlane(ids[i]), first));
+        } else {
+          from = reinterpret_cast<const char*>(base + (int64_t)key0 * stride);
+        }
+        unsigned at = off[i];
+        if (!whole) at -= (unsigned)(max(first + (PAGED ? lane / CH : piece_row(i)) - (w.keys - 1), 0) * (int)stride * (int)sizeof(T));
+        src = from + at;
       }
       __builtin_amdgcn_global_load_lds(KX_CKN(a, is_k ? PP_K : PP_V, src, 16),
-                                       (lds_ptr)(smem + buf * 2 * TILEB + (wave + NW * i) * 1024), 16, 0, 0);
+                                       (lds_ptr)(smem + buf * KG * 2 * TILEB + (wave + NW * i) * 1024), 16, 0, 0);
     }
   };
 
   if (t0 < t1) {
     get_ids(t0);
     issue_tile(t0, 0);
-    if (t0 + 1 < t1) get_ids(t0 + 1);
+    if (t0 + KG < t1) get_ids(t0 + KG);
   }
   // a page that is not there: looked for once, and tile by tile only if there is one
   bool missing = false;
@@ -272,32 +319,49 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, key0 = t * kPaKeys;
-    if (t + 1 < t1) {
-      issue_tile(t + 1, buf ^ 1);
-      if (t + 2 < t1) get_ids(t + 2);
+  for (int t = t0, buf = 0; t < t1; t += KG, buf ^= 1) {
+    if (t + KG < t1) {
+      issue_tile(t + KG, buf ^ 1);
+      if (t + 2 * KG < t1) get_ids(t + 2 * KG);
     }
-    if (key0 < w_hi && key0 + kPaKeys > w_lo) {
-      const lds_bytes base = (lds_bytes)smem + buf * 2 * TILEB;
+    const int key0 = (t + group) * KT;  // this wave's tile
+    if (key0 < w_hi && key0 + KT > w_lo) {
+      const lds_bytes base = (lds_bytes)smem + (buf * KG + group) * 2 * TILEB;
       // ---- scores: register r of s[kt] is key 32 kt + 8 (r / 4) + 4 half + r % 4 ----
-      f32x16 s[2];
+      f32x16 s[KT / 32];
+      {
+        frag kf[KT / 32][KS];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < KT / 32; ++kt) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+          for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const frag kf = *(const __attribute__((address_space(3))) frag*)(base + kfrag[ks] + kt * 32 * ROWB);
-          if constexpr (F32) {
+          for (int ks = 0; ks < KS; ++ks)
+            kf[kt][ks] = *(const __attribute__((address_space(3))) frag*)(base + kfrag[ks] + kt * 32 * ROWB);
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[ks][e], s[kt], 0, 0, 0);
-          } else {
-            s[kt] = PromptMma<T>::mul(kf, qf[ks], s[kt]);
+        for (int kt = 0; kt < KT / 32; ++kt)
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (F32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[kt][ks][e], qf[ks][e], s[kt], 0, 0, 0);
+            } else {
+              s[kt] = PromptMma<T>::mul(kf[kt][ks], qf[ks], s[kt]);
+            }
           }
+        if constexpr (!F32) {
+          // half of the fragments ahead of the first product, then one read behind each product
+          __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
         }
       }
-      if (key0 + kPaKeys > full_hi || key0 < full_lo || missing) {
+      if (key0 + KT > full_hi || key0 < full_lo || missing) {
         unsigned long long there = ~0ull;
         if (PAGED && missing) {
           const int at = key0 + lane;
@@ -305,7 +369,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
         }
         there >>= 4 * half;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < KT / 32; ++kt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int k = 32 * kt + 8 * (r / 4) + r % 4, at = key0 + k + 4 * half;
@@ -314,7 +378,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
       }
       float mx = s[0][0];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < KT / 32; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
       mx = xor32_max(mx);
@@ -331,7 +395,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
       }
       const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int kt = 0; kt < KT / 32; ++kt) {
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -348,8 +412,6 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
               o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[kt][r], o[dt], 0, 0, 0);
             }
         } else {
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
 #pragma unroll
           for (int st = 0; st < 2; ++st) {
             frag pf;
@@ -357,10 +419,9 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
             for (int j = 0; j < 8; ++j) pf[j] = (T)s[kt][8 * st + j];
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-              typedef __attribute__((address_space(3))) s16x4* tr_ptr;
               const lds_bytes at = base + vfrag[dt] + (32 * kt + 16 * st) * ROWB;
-              const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
-              const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 8 * ROWB));
+              const s16x4 lo4 = read_transposed((lds_tr_ptr)at);
+              const s16x4 hi4 = read_transposed((lds_tr_ptr)(at + 8 * ROWB));
               const s16x8 both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
               o[dt] = PromptMma<T>::mul(__builtin_bit_cast(frag, both), pf, o[dt]);
             }
@@ -371,13 +432,53 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
+  l = xor32_sum(l);
+  if constexpr (KG > 1) {
+    // the groups' results meet in LDS (nothing of the tiles is read any more)
+    constexpr int PART = (DT * 16 + 2) * 64 * 4;  // bytes of a wave's o, m, l
+    static_assert((KG - 1) * PW * PART <= 2 * KG * 2 * TILEB, "");
+    if (group > 0) {
+      char* mine = smem + (wave - PW) * PART;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(mine + ((dt * 4 + q) * 64 + lane) * 16) =
+              f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+      *reinterpret_cast<float*>(mine + DT * 16 * 64 * 4 + lane * 4) = m;
+      *reinterpret_cast<float*>(mine + (DT * 16 + 1) * 64 * 4 + lane * 4) = l;
+    }
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < KG; ++g) {
+      const char* part = smem + ((g - 1) * PW + wave) * PART;
+      const float pm = *reinterpret_cast<const float*>(part + DT * 16 * 64 * 4 + lane * 4);
+      const float pl = *reinterpret_cast<const float*>(part + (DT * 16 + 1) * 64 * 4 + lane * 4);
+      const float m_new = fmaxf(m, pm);
+      // a part without a maximum holds zeros, or NaN: those stay
+      const float fa = m == m_new ? 1.f : m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+      const float fb = pm == m_new ? 1.f : pm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm - m_new) * c);
+      l = l * fa + pl * fb;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 po = *reinterpret_cast<const f32x4*>(part + ((dt * 4 + q) * 64 + lane) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = o[dt][4 * q + e] * fa + po[e] * fb;
+        }
+      m = m_new;
+    }
+  }
   if (wf0 >= pairs) return;
 
   // ---- results: through the wave's part of LDS to whole rows ----
-  l = xor32_sum(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float odd = 0.f;  // NaN if any result is not finite
-  char* region = smem + wave * 32 * ROWB;
+  // (with groups: where the first of the parts that this wave alone has read lies)
+  char* region = smem + wave * (KG > 1 ? (DT * 16 + 2) * 256 : 32 * ROWB);
+  static_assert((DT * 16 + 2) * 256 >= 32 * ROWB, "");
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -467,28 +568,53 @@ __global__ __launch_bounds__(NW * 64, 2) void prompt_attn_kernel(const PromptArg
   }
 }
 
-template <typename T, int HS, int MODE, int NW>
+// the two buffers; the rows of the results pass through the same place
+template <typename T, int HS, int KG>
+constexpr int prompt_lds() {
+  const int row = HS * (int)sizeof(T), tiles = 2 * KG * 2 * pa_keys<T>() * row, rows = KG == 1 ? kPaWaves * 32 * row : 0;
+  return tiles > rows ? tiles : rows;
+}
+
+template <typename T, int HS, int MODE, int KG>
 static int prompt_launch(const PromptArgs& a, hipStream_t s) {
-  constexpr int lds = 2 * 2 * kPaKeys * HS * (int)sizeof(T);
+  constexpr int pairs = kPaWaves / KG * 32, lds = prompt_lds<T, HS, KG>();
   static OncePerDevice limit;
   if (lds > 32768)
-    if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, NW>), lds)) return rc;
+    if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, KG>), lds)) return rc;
   // blocks of the sequences: an even share of all pairs and one more each
-  const int64_t items = (int64_t)a.q_rows * a.kv_mul / (NW * 32) + a.batch;
+  const int64_t items = (int64_t)a.q_rows * a.kv_mul / pairs + a.batch;
   if (items * a.kv_heads > 0x7fffffffll) return KX_ELIMIT;
-  hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, NW>), dim3((unsigned)(items * a.kv_heads)), dim3(NW * 64), lds, s, a);
+  hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, KG>), dim3((unsigned)(items * a.kv_heads)), dim3(kPaWaves * 64), lds, s, a);
   KX_LAUNCH_CHECK();
   return KX_OK;
 }
-template <typename T, int HS>
+template <typename T, int HS, int KG>
 static int prompt_mode(const PromptArgs& a, hipStream_t s) {
-  if (!a.kv.table) return prompt_launch<T, HS, PA_PACKED, 8>(a, s);
-  if (a.kv.div.size % 16 == 0) return prompt_launch<T, HS, PA_BLOCK_PAGES, 8>(a, s);
-  return prompt_launch<T, HS, PA_ANY_PAGES, 8>(a, s);
+  if (!a.kv.table) return prompt_launch<T, HS, PA_PACKED, KG>(a, s);
+  if (a.kv.div.size % 16 == 0) return prompt_launch<T, HS, PA_BLOCK_PAGES, KG>(a, s);
+  return prompt_launch<T, HS, PA_ANY_PAGES, KG>(a, s);
+}
+// Groups of waves per workgroup.  Two or more cut a sequence's chain of tiles and give that many times the workgroups, for
+// as many times the K/V traffic per product.
+//   16-bit: two groups where the call would not fill the chip with workgroups of 256 pairs (`blocks`) otherwise: under 320
+//   of them, or under 800 with 64-wide heads, whose smaller tiles let two such workgroups share a CU.  Measured (us,
+//   one group / two; causal, 32 heads over 8): 128 wide, blocks 64: 20.1 / 16.2, 256: 61.2 / 52.8, 375: 93 / 105, 512 (a
+//   prompt of 4096): 134 / 155; 64 wide, 128: 23.3 / 15.9, 473: 35.2 / 31.6, 1382: 103 / 116; 32 wide, 74: 35.2 / 21.1, 674:
+//   51.7 / 57.8.
+//   fp32: as many groups as LDS holds buffers for, always: its products take sixteen times as long and hide the traffic
+//   (64 wide, blocks 31: one 33.7, two 26.8, four 18.9; 612: one 367, four 303; 128 wide, 512: one 1145, two 1097).
+template <typename T, int HS>
+static int prompt_groups(const PromptArgs& a, hipStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    return prompt_mode<T, HS, prompt_lds<T, HS, 4>() <= 131072 ? 4 : 2>(a, s);
+  } else {
+    const double blocks = (double)a.q_rows * a.kv_mul / 256 * a.kv_heads;
+    return blocks < (HS == 64 ? 800 : 320) ? prompt_mode<T, HS, 2>(a, s) : prompt_mode<T, HS, 1>(a, s);
+  }
 }
 template <typename T>
 static int prompt_hs(const PromptArgs& a, int hs, hipStream_t s) {
-  return hs == 32 ? prompt_mode<T, 32>(a, s) : hs == 64 ? prompt_mode<T, 64>(a, s) : prompt_mode<T, 128>(a, s);
+  return hs == 32 ? prompt_groups<T, 32>(a, s) : hs == 64 ? prompt_groups<T, 64>(a, s) : prompt_groups<T, 128>(a, s);
 }
 
 }  // namespace kx
@@ -519,8 +645,8 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
     if (!d->k || !d->v || !d->cu_k || (uintptr_t)d->cu_k % 4 || d->k_rows < 0 || !aligned16(d->k) || !aligned16(d->v) ||
         !stride_ok(d->k_stride, kv_dim, unit) || !stride_ok(d->v_stride, kv_dim, unit))
       return KX_EINVAL;
-    // a tile's rows are addressed by 31-bit offsets from its first one
-    if ((uint64_t)d->k_stride * bytes * kPaKeys > 0x7fffffffull || (uint64_t)d->v_stride * bytes * kPaKeys > 0x7fffffffull)
+    // the rows of a buffer (256 keys at most) are addressed by 31-bit offsets from the first one
+    if ((uint64_t)d->k_stride * bytes * 256 > 0x7fffffffull || (uint64_t)d->v_stride * bytes * 256 > 0x7fffffffull)
       return KX_EUNSUPPORTED;
     a.k = static_cast<const char*>(d->k);
     a.v = static_cast<const char*>(d->v);
