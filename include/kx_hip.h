@@ -624,8 +624,8 @@ typedef struct kx_paged_kv {
  * q_out: KX_F32 into any cache, KX_F16 / KX_BF16 into a cache of the same type.  A row whose position
  * is outside 0 .. table_pages * page_size - 1, has no page or (when rotating) lies past table_rows is not filed; past
  * table_rows or below zero its q row is left alone too.  Rows of no sequence (below cu_rows[0], from cu_rows[batch] on) are left
- * alone.  No two rows of a call may have the same place in the pages.  Strides in elements, multiples of 4 and
- * at least the row's width; pointers aligned to 16 bytes (KX_EINVAL). */
+ * alone.  No two rows of a call may have the same place in the pages.  Strides in elements, at least the
+ * row's width and multiples of 16 bytes; pointers aligned to 16 bytes (KX_EINVAL). */
 typedef struct kx_paged_write_desc {
   kx_paged_kv kv;
   int32_t src_type;

@@ -6,7 +6,7 @@
 // Bound: the row is read once (rows * vocab * element size); about ten vector instructions per element, four of them the
 // exponential, are three quarters of that time for 16-bit logits.
 //
-// Split: a workgroup takes a row, or with few rows one of up to 64 parts of it; the parts' sums and lists meet in the
+// Split: a workgroup takes a row, or with few rows one of up to 32 parts of it; the parts' sums and lists meet in the
 // workspace and the workgroup that arrives last joins them in their order.
 //
 // Alternatives without a second pass: a lane keeps its largest value of all and of each of eight groups of its loads.  The
@@ -29,7 +29,7 @@ constexpr int kLpThreads = 256, kLpWaves = kLpThreads / 64;
 constexpr int kLpUnroll = 4;      // vectors of 16 bytes in flight per lane
 constexpr int kLpGroups = 8;      // groups of a lane's loads
 constexpr int kLpList = 512;      // elements that are ranked at once
-constexpr int kLpMaxParts = 64;   // one lane each in the join
+constexpr int kLpMaxParts = 32;   // of a row
 constexpr int kLpSlots = 1024;    // workgroups that few rows are cut for
 constexpr int kLpRecord = 16 + 8 * KX_LOGPROBS_TOP_MAX;  // bytes: m, z, s, -, then the list
 constexpr size_t kLpTicketBytes = (size_t)kLpSlots * 64;
@@ -48,35 +48,32 @@ struct LogprobsArgs {
   KX_BFIELD(7)
 };
 
+// fp32 values as whole numbers of the same order
+__device__ __forceinline__ unsigned order_of(float x) {
+  const unsigned u = __float_as_uint(x);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of_order(unsigned u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
+
+// At most the n-th largest of the wave's values: its first 20 bits, found from the top (0 with fewer than n above it).
+__device__ __forceinline__ unsigned nth_largest(unsigned v, int n) {
+  unsigned t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 12; --bit) {
+    const unsigned c = t | 1u << bit;
+    if (__builtin_popcountll(__ballot(v >= c)) >= n) t = c;
+  }
+  return t;
+}
+
 // Order of the alternatives as an unsigned whole number: larger value first, the lower index ahead among equal ones
 // (both zeros are equal), NaN below -inf.  No element has key 0.
 __device__ __forceinline__ unsigned long long key_of(float x, int index) {
-  unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
-  u = u >> 31 ? ~u : u | 0x80000000u;
-  if (x != x) u = 0u;
+  const unsigned u = x != x ? 0u : order_of(x == 0.f ? 0.f : x);
   return (unsigned long long)u << 32 | (0xffffffffu - (unsigned)index);
 }
-__device__ __forceinline__ float value_of_key(unsigned long long k) {
-  const unsigned u = (unsigned)(k >> 32);
-  return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
-}
+__device__ __forceinline__ float value_of_key(unsigned long long k) { return value_of_order((unsigned)(k >> 32)); }
 __device__ __forceinline__ int index_of_key(unsigned long long k) { return (int)(0xffffffffu - (unsigned)k); }
-
-__device__ __forceinline__ unsigned umax_dpp_row(unsigned v) {
-  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
-  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
-  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
-  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
-}
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-  v = umax_dpp_row(v);
-  unsigned a = v, b = v;
-  permlane16_swap(a, b);
-  v = max(a, b);
-  a = v, b = v;
-  permlane32_swap(a, b);
-  return max(a, b);
-}
 
 template <typename T> struct LogitVec;  // 16 bytes of logits
 template <> struct LogitVec<float> {
@@ -118,6 +115,7 @@ __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int co
   for (int i = threadIdx.x; i < count; i += kLpThreads) {
     const unsigned long long mine = keys[i];
     int above = 0;
+#pragma unroll 8
     for (int j = 0; j < count; ++j) above += keys[j] > mine;
     if (above < top_n) out[above] = mine;
   }
@@ -127,8 +125,10 @@ template <typename T>
 __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsArgs a) {
   typedef LogitVec<T> Vec;
   constexpr int N = Vec::N;
-  // group maxima and the list; in the join the parts' lists
-  __shared__ __attribute__((aligned(16))) unsigned long long sm_raw[kLpMaxParts * KX_LOGPROBS_TOP_MAX];
+  // group maxima and the list; in the join the parts' lists, and those of their keys that may be among the best: the
+  // lists of top_n parts at most
+  __shared__ __attribute__((aligned(16))) unsigned long long sm_raw[2 * kLpMaxParts * KX_LOGPROBS_TOP_MAX];
+  unsigned long long* sm_best = sm_raw + kLpMaxParts * KX_LOGPROBS_TOP_MAX;
   static_assert(sizeof(sm_raw) >= kLpGroups * kLpThreads * 4 + kLpList * 8, "");
   float* sm_group = reinterpret_cast<float*>(sm_raw);
   unsigned long long* sm_list = sm_raw + kLpGroups * kLpThreads / 2;
@@ -173,11 +173,11 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     }
   };
   int step = 0;
+  u32x4 v[kLpUnroll];  // (fp32: the elements of an only step stay for the search below)
   for (int group = 0; step < steps; ++group) {
     float group_max = -INFINITY;
     const int end = min(step + group_steps, steps);
     for (; step < end; ++step) {
-      u32x4 v[kLpUnroll];
       load_step(step, v);
       float mx = Vec::get(v[0], 0);
 #pragma unroll
@@ -214,15 +214,9 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     sm_sums[wave][2] = sums.s;
   }
   if (a.top_n > 0) {
-    // the top_n-th largest of the lanes' maxima, the lower lane ahead among equal ones
-    int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < 64; ++j) {
-      const float other = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(largest), j));
-      above += other > largest || (other == largest && j < lane);
-    }
-    const unsigned long long at = __ballot(above == a.top_n - 1);
-    if (lane == 0) sm_least[wave] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(largest), __builtin_ctzll(at)));
+    // (a bound below every value is a NaN here, which no value is below)
+    const float bound = value_of_order(nth_largest(order_of(largest), a.top_n));
+    if (lane == 0) sm_least[wave] = bound;
   }
   __syncthreads();
   LogSums all = {-INFINITY, 0.f, 0.f};
@@ -240,24 +234,38 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     float least = sm_least[0];
 #pragma unroll
     for (int w = 1; w < kLpWaves; ++w) least = fmaxf(least, sm_least[w]);
-    auto take = [&](float v, int index) {
-      if (v < least) return;  // (NaN stays: it may be among the best of a row with less than top_n others)
+    // not below it (a NaN may be among the best of a row with fewer than top_n others)
+    if (extra >= 0 && !(xe < least)) {
       const int at = atomicAdd(&sm_count, 1);
-      if (at < kLpList) sm_list[at] = key_of(v, index);
-    };
-    if (extra >= 0) take(xe, extra);
+      if (at < kLpList) sm_list[at] = key_of(xe, extra);
+    }
     for (int group = 0; group * group_steps < steps; ++group) {
       if (sm_group[group * kLpThreads + tid] < least) continue;
       for (int st = group * group_steps; st < min((group + 1) * group_steps, steps); ++st) {
-        u32x4 v[kLpUnroll];
-        load_step(st, v);
+        // fp32: the whole step, which is still at hand if it is the only one; 16-bit types: a vector at a time (registers
+        // are dearer than the wait)
+        constexpr int AT_ONCE = N == 4 ? kLpUnroll : 1;
+#pragma unroll 1
+        for (int u0 = 0; u0 < kLpUnroll; u0 += AT_ONCE) {
+          const int first = v0 + st * per_step + u0 * kLpThreads + tid;
+          if (N == 8) v[0] = *KX_CK(a, PL_X, xv + min(first, v1 - 1));
+          else if (steps > 1) load_step(st, v);
+          unsigned hits = 0;
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
-          const int i = v0 + st * per_step + u * kLpThreads + tid;
-          if (i < v1) {
+          for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-            for (int e = 0; e < N; ++e) take(Vec::get(v[u], e), ahead + i * N + e);
-          }
+            for (int e = 0; e < N; ++e)
+              if (!(Vec::get(v[u], e) < least) && first + u * kLpThreads < v1) hits |= 1u << (u * N + e);
+          if (!hits) continue;
+          int at = atomicAdd(&sm_count, __builtin_popcount(hits));
+#pragma unroll
+          for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (hits >> (u * N + e) & 1) {
+                if (at < kLpList) sm_list[at] = key_of(Vec::get(v[u], e), ahead + (first + u * kLpThreads) * N + e);
+                ++at;
+              }
         }
       }
     }
@@ -314,31 +322,41 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     __syncthreads();
     if (!sm_last) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    for (int i = tid; i < a.parts * a.top_n; i += kLpThreads) {
-      const int p = i / a.top_n;
-      const u32x2 k = __builtin_amdgcn_raw_buffer_load_b64(rec, p * kLpRecord + 16 + 8 * (i - p * a.top_n), 0, 16);
-      sm_raw[i] = (unsigned long long)k.y << 32 | k.x;
+    // the parts' lists, all requested before the first is used
+    constexpr int ROUNDS = kLpMaxParts * KX_LOGPROBS_TOP_MAX / kLpThreads;
+    const int keys = a.parts * a.top_n;
+    u32x2 k[ROUNDS];
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j) {
+      const int i = max(min(tid + j * kLpThreads, keys - 1), 0), p = a.top_n ? i / a.top_n : 0;
+      k[j] = __builtin_amdgcn_raw_buffer_load_b64(rec, p * kLpRecord + 16 + 8 * (i - p * a.top_n), 0, 16);
     }
     const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(rec, min(lane, a.parts - 1) * kLpRecord, 0, 16);
     LogSums one = {__uint_as_float(s.x), __uint_as_float(s.y), __uint_as_float(s.z)};
     if (lane >= a.parts) one = LogSums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < ROUNDS; ++j)
+      if (tid + j * kLpThreads < keys) sm_raw[tid + j * kLpThreads] = (unsigned long long)k[j].y << 32 | k[j].x;
     const float m = wave_max(one.m);
     rebase(one, m);
     all = LogSums{m, wave_sum(one.z), wave_sum(one.s)};
+    if (tid == 0) sm_count = 0;
     __syncthreads();
-    if (wave != 0) return;
-    // the parts' lists fall: take the largest head top_n times, lane p at part p's list
-    int at = 0;
-    unsigned long long head = lane < a.parts && a.top_n > 0 ? sm_raw[lane * a.top_n] : 0;
-    for (int n = 0; n < a.top_n; ++n) {
-      const unsigned hi = wave_umax((unsigned)(head >> 32));
-      const unsigned lo = wave_umax((unsigned)(head >> 32) == hi ? (unsigned)head : 0u);
-      const unsigned long long top = (unsigned long long)hi << 32 | lo;
-      if (lane == n) best = top;
-      if (head == top) {
-        ++at;
-        head = at < a.top_n ? sm_raw[lane * a.top_n + at] : 0;
+    if (a.top_n > 0) {
+      // The parts' lists fall.  With `depth` keys of each list at least top_n: no key below all of those is among the best;
+      // with a head of top_n lists or more, none below the top_n-th largest of the heads.
+      const int depth = (a.top_n + a.parts - 1) / a.parts;
+      const unsigned head = lane < a.parts ? (unsigned)(sm_raw[lane * a.top_n + depth - 1] >> 32) : 0u;
+      const unsigned long long bound = (unsigned long long)nth_largest(head, depth == 1 ? a.top_n : a.parts) << 32;
+#pragma unroll
+      for (int j = 0; j < ROUNDS; ++j) {
+        const unsigned long long key = (unsigned long long)k[j].y << 32 | k[j].x;
+        if (tid + j * kLpThreads < keys && key >= bound) sm_best[atomicAdd(&sm_count, 1)] = key;
       }
+      __syncthreads();
+      rank_keys(sm_best, sm_count, a.top_n, sm_top);
+      __syncthreads();
+      best = tid < a.top_n ? sm_top[tid] : 0;
     }
   }
   if (wave != 0) return;

@@ -37,7 +37,7 @@ def exact_attention(q, k, v, seen, scale):
         p /= p.sum()
         out[i] = p @ v[at]
         spread[i] = p @ np.abs(v[at])
-        size[i] = 8 * np.sqrt(q.shape[1]) * U * (scale * (np.abs(k[at]) @ np.abs(q[i]))).max() + 8 * np.sqrt(len(at)) * U
+        size[i] = 8 * np.sqrt(q.shape[1]) * U * (abs(scale) * (np.abs(k[at]) @ np.abs(q[i]))).max() + 8 * np.sqrt(len(at)) * U
     return out, spread, size
 
 
@@ -263,6 +263,17 @@ def test_decode_large_scores_and_values(q_kind, kind):
     check_decode(cache, q, got, 0, 1 / np.sqrt(128), q_kind)
 
 
+@pytest.mark.parametrize("q_kind,kind", KINDS, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+def test_decode_scales(q_kind, kind, scale):
+    rng = np.random.default_rng(10)
+    lens = [77, 1, 300]
+    cache = Cache(rng, lens, 2, 64, 16, kind)
+    q = rounded(rng.standard_normal((3, 6, 64)).astype(np.float32), q_kind)
+    got = kx.paged_decode(cache.pool, cache.table, lens, q, scale=scale, window=50, q_kind=q_kind)
+    check_decode(cache, q, got, 50, scale, q_kind)
+
+
 def test_decode_offsets_past_32_bits():
     """A pool of more than 2^31 elements: the last pages are reached (rows sit at a page stride of 2^26 elements)."""
     pages, stride, hs = 70, 1 << 26, 128
@@ -446,6 +457,16 @@ def test_prompt_rows_do_not_see_what_is_masked(kind):
     check_prompt(q[:90], [0, 90], [k[:90]], [v[:90]], got[:90], kind, 0.125)
     assert np.isposinf(got[90:97, 2:, 5]).all() and np.isfinite(got[90:97, :2]).all()
     assert np.isnan(got[97:, :2]).all() and np.isnan(got[100:]).all()
+
+
+@pytest.mark.parametrize("kind", [kx.F32, kx.F16, kx.BF16], ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 1.0])
+def test_prompt_scales(kind, scale):
+    rng = np.random.default_rng(42)
+    cu = [0, 100, 133]
+    q, k, v = (rounded(rng.standard_normal((133, m, 64)).astype(np.float32), kind) for m in (4, 2, 2))
+    got = kx.prompt_attention(q, cu, k, v, scale=scale, window=70, kind=kind)
+    check_prompt(q, cu, [k[:100], k[100:]], [v[:100], v[100:]], got, kind, scale, True, 70)
 
 
 @pytest.mark.parametrize("kind", [kx.F16, kx.BF16, kx.F32], ids=lambda k: NAMES[k])
