@@ -128,11 +128,12 @@ __device__ __forceinline__ int v_swizzle(int row) {
 }
 
 // A transposing LDS read: of the 4 rows x 16 elements that 16 lanes point at (8 bytes each, row i / 4 for lane i), lane i
-// gets column i.
+// gets column i.  The restrict pointer tells the compiler that the read does not meet the LDS-DMA in flight (it fills
+// the other buffer); without it every such read waits for all of that first.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4* lds_tr_ptr;
-__device__ __forceinline__ s16x4 read_transposed(lds_tr_ptr p) {
+__device__ __forceinline__ s16x4 read_transposed(lds_tr_ptr __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
 }
 
@@ -164,12 +165,12 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
   constexpr int RPP = 1024 / ROWB;               // rows per DMA instruction
   constexpr int TILEB = KT * ROWB;               // K (or V) bytes of a tile
   constexpr int KP = TILEB / 1024;               // DMA instructions for them
-  constexpr int PER = 2 * KP * KG / NW;          // per wave and buffer
+  constexpr int RP = (KP * KG + NW - 1) / NW;    // of K (and of V) per wave and buffer
   constexpr int DT = HS / 32;                    // output tiles
   // fp16 weights are held 2^7 times as large: at most 2^15, and whole down to 2^-21 of the largest
   constexpr float kShift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
   constexpr int KS = HS * (int)sizeof(T) / 32;   // 32-byte steps of the first product
-  static_assert(2 * KP * KG % NW == 0, "");
+  static_assert(KP * KG % NW == 0 || KP * KG < NW, "");
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers of KG tiles, K and V each
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef const __attribute__((address_space(3))) char* lds_bytes;
@@ -203,72 +204,83 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
   const int32_t* table = PAGED ? a.kv.table + w.b * a.kv.table_stride : nullptr;
   auto page_ok = [&](int p) { return (unsigned)p < (unsigned)a.kv.num_pages; };
   auto lookup = [&](int t) { return *KX_CK(a, PP_TABLE, table + a.kv.div.page(t)); };
-  auto paged_row = [&](const T* base, int page, int t) {
-    return base + (page_ok(page) ? page : 0) * a.kv.page_stride + (t - a.kv.div.page(t) * a.kv.div.size) * a.kv.row_stride;
+  const unsigned page_bytes = PAGED ? (unsigned)(a.kv.page_stride * sizeof(T)) : 0u, row_bytes = PAGED ? (unsigned)(a.kv.row_stride * sizeof(T)) : 0u;
+  // byte offset of position t, whose page is `page` (one that is not there: some page that is)
+  auto paged_offset = [&](int page, int t) {
+    return (uint64_t)(page_ok(page) ? (unsigned)page : 0u) * page_bytes +
+           (uint64_t)(unsigned)(t - a.kv.div.page(t) * a.kv.div.size) * row_bytes;
   };
-  // The KG tiles of a buffer are consecutive, so its K rows are KG * KT consecutive keys.  DMA instruction q of a
-  // buffer: tile q / (2 KP), K rows then V rows; the first of its rows among the keys, and a lane's.
-  auto piece_first = [&](int i) { return (wave + NW * i) / (2 * KP) * KT + (wave + NW * i) % KP * RPP; };
-  auto piece_row = [&](int i) { return piece_first(i) + lane / CH; };
-  auto piece_is_k = [&](int i) { return (wave + NW * i) % (2 * KP) < KP; };
-  // a lane's byte offset from the first row of the buffer (packed), from the first row of the instruction's 16-row block,
-  // or within its row (pages)
-  unsigned off[PER];
+  // The KG tiles of a buffer are consecutive, so its K rows are KG * KT consecutive keys.  DMA pair j of a wave, one
+  // instruction for K and one for V: the first of its rows among the keys, and a lane's.
+  auto pair_first = [&](int j) { return (wave + NW * j) * RPP; };
+  auto pair_row = [&](int j) { return pair_first(j) + lane / CH; };
+  const bool has_pair = KP * KG >= NW || wave < KP * KG;
+  // a lane's byte offsets from the first row of the buffer (packed), from the first row of the instruction's 16-row block, or
+  // within its row (pages); `tail`: those in the last buffer, where rows behind the last key are replaced by it
+  unsigned k_off[RP], v_off[RP], k_tail[RP], v_tail[RP];
+  const int steps = (t1 - t0 + KG - 1) / KG, tail_key0 = (t0 + (steps - 1) * KG) * KT;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = piece_row(i), from = MODE == PA_PACKED ? row : MODE == PA_BLOCK_PAGES ? lane / CH : 0;
-    off[i] = 16u * (lane % CH ^ (piece_is_k(i) ? k_swizzle<CH>(row) : v_swizzle<CH, F32>(row))) +
-             (unsigned)(from * (int)(piece_is_k(i) ? k_stride : v_stride) * (int)sizeof(T));
+  for (int j = 0; j < RP; ++j) {
+    const int row = pair_row(j), from = MODE == PA_PACKED ? row : MODE == PA_BLOCK_PAGES ? lane / CH : 0;
+    const int block = min(tail_key0 + pair_first(j), (w.keys - 1) & ~(RPP - 1)) + lane / CH;
+    const int behind = MODE == PA_PACKED ? max(tail_key0 + row - (w.keys - 1), 0) : MODE == PA_BLOCK_PAGES ? max(block - (w.keys - 1), 0) : 0;
+    const unsigned kp = 16u * (lane % CH ^ k_swizzle<CH>(row)), vp = 16u * (lane % CH ^ v_swizzle<CH, F32>(row));
+    const unsigned kb = (unsigned)((int)k_stride * (int)sizeof(T)), vb = (unsigned)((int)v_stride * (int)sizeof(T));
+    k_off[j] = kp + from * kb;
+    v_off[j] = vp + from * vb;
+    k_tail[j] = kp + (unsigned)(from - behind) * kb;
+    v_tail[j] = vp + (unsigned)(from - behind) * vb;
   }
   // Pages of the next buffer's rows, requested a step ahead: one per instruction where pages are whole 16-row blocks, else
   // one per lane.  (By vector loads in both cases: the end of a step waits for those anyway, while a scalar load would
   // have the next fragment reads wait for it.)
-  int ids[PAGED ? PER : 1];
+  int ids[PAGED ? RP : 1];
   auto get_ids = [&](int t) {
     if constexpr (PAGED) {
       int zero;
       asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
+      for (int j = 0; j < RP; ++j) {
         if constexpr (MODE == PA_BLOCK_PAGES)
-          ids[i] = lookup(min(t * KT + piece_first(i), (w.keys - 1) & ~(RPP - 1)) + zero);
+          ids[j] = lookup(min(t * KT + pair_first(j), (w.keys - 1) & ~(RPP - 1)) + zero);
         else
-          ids[i] = lookup(min(t * KT + piece_row(i), w.keys - 1));
+          ids[j] = lookup(min(t * KT + pair_row(j), w.keys - 1));
       }
     }
   };
-  auto issue_tile = [&](int t, int buf) {
+  auto issue = [&](int t, int buf, int from, int upto) {
+    if (!has_pair) return;
     const int key0 = t * KT;
-    const bool whole = key0 + KG * KT <= w.keys;  // else rows behind the last are replaced by it
+    const bool whole = key0 + KG * KT <= w.keys;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bool is_k = piece_is_k(i);
-      const T* base = is_k ? kbase : vbase;
-      const char* src;
+    for (int j = 0; j < RP; ++j) {
+      if (j < from || j >= upto) continue;
+      const char* ks = reinterpret_cast<const char*>(kbase);
+      const char* vs = reinterpret_cast<const char*>(vbase);
       if constexpr (MODE == PA_ANY_PAGES) {
-        src = reinterpret_cast<const char*>(paged_row(base, ids[i], min(key0 + piece_row(i), w.keys - 1))) + off[i];
+        const uint64_t at = paged_offset(ids[j], min(key0 + pair_row(j), w.keys - 1));
+        ks += at;
+        vs += at;
+      } else if constexpr (MODE == PA_BLOCK_PAGES) {
+        const uint64_t at = paged_offset(__builtin_amdgcn_readfirstlane(ids[j]), min(key0 + pair_first(j), (w.keys - 1) & ~(RPP - 1)));
+        ks += at;
+        vs += at;
       } else {
-        const int64_t stride = is_k ? k_stride : v_stride;
-        int first = key0;  // uniform
-        const char* from;
-        if constexpr (MODE == PA_BLOCK_PAGES) {
-          first = min(key0 + piece_first(i), (w.keys - 1) & ~(RPP - 1));
-          from = reinterpret_cast<const char*>(paged_row(base, __builtin_amdgcn_readfirstlane(ids[i]), first));
-        } else {
-          from = reinterpret_cast<const char*>(base + (int64_t)key0 * stride);
-        }
-        unsigned at = off[i];
-        if (!whole) at -= (unsigned)(max(first + (PAGED ? lane / CH : piece_row(i)) - (w.keys - 1), 0) * (int)stride * (int)sizeof(T));
-        src = from + at;
+        ks += (int64_t)key0 * k_stride * (int)sizeof(T);
+        vs += (int64_t)key0 * v_stride * (int)sizeof(T);
       }
-      __builtin_amdgcn_global_load_lds(KX_CKN(a, is_k ? PP_K : PP_V, src, 16),
-                                       (lds_ptr)(smem + buf * KG * 2 * TILEB + (wave + NW * i) * 1024), 16, 0, 0);
+      ks += whole ? k_off[j] : k_tail[j];
+      vs += whole ? v_off[j] : v_tail[j];
+      const int q = wave + NW * j;
+      char* to = smem + buf * KG * 2 * TILEB + q / KP * 2 * TILEB + q % KP * 1024;
+      __builtin_amdgcn_global_load_lds(KX_CKN(a, PP_K, ks, 16), (lds_ptr)to, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(KX_CKN(a, PP_V, vs, 16), (lds_ptr)(to + TILEB), 16, 0, 0);
     }
   };
 
   if (t0 < t1) {
     get_ids(t0);
-    issue_tile(t0, 0);
+    issue(t0, 0, 0, RP);
     if (t0 + KG < t1) get_ids(t0 + KG);
   }
   // a page that is not there: looked for once, and tile by tile only if there is one
@@ -320,47 +332,50 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   for (int t = t0, buf = 0; t < t1; t += KG, buf ^= 1) {
-    if (t + KG < t1) {
-      issue_tile(t + KG, buf ^ 1);
-      if (t + 2 * KG < t1) get_ids(t + 2 * KG);
-    }
+    // The next tiles are requested in two parts beside the scores: the LDS-DMA of a CU takes 64 bytes a cycle, and a wave
+    // that sends all of its share at once waits for that.
+    const bool more = t + KG < t1;
     const int key0 = (t + group) * KT;  // this wave's tile
     if (key0 < w_hi && key0 + KT > w_lo) {
       const lds_bytes base = (lds_bytes)smem + (buf * KG + group) * 2 * TILEB;
       // ---- scores: register r of s[kt] is key 32 kt + 8 (r / 4) + 4 half + r % 4 ----
       f32x16 s[KT / 32];
-      {
-        frag kf[KT / 32][KS];
+      frag kf[KT / 32][KS];
 #pragma unroll
-        for (int kt = 0; kt < KT / 32; ++kt) {
+      for (int kt = 0; kt < KT / 32; ++kt) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            kf[kt][ks] = *(const __attribute__((address_space(3))) frag*)(base + kfrag[ks] + kt * 32 * ROWB);
+        for (int ks = 0; ks < KS; ++ks)
+          kf[kt][ks] = *(const __attribute__((address_space(3))) frag*)(base + kfrag[ks] + kt * 32 * ROWB);
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT / 32; ++kt) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[kt][ks][e], qf[ks][e], s[kt], 0, 0, 0);
+          } else {
+            s[kt] = PromptMma<T>::mul(kf[kt][ks], qf[ks], s[kt]);
+          }
         }
+        if constexpr (!F32) {
+          if (kt == 0) {
+            // half of the fragments ahead of the first product, then one read behind each product
+            __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
 #pragma unroll
-        for (int kt = 0; kt < KT / 32; ++kt)
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (F32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[kt][ks][e], qf[ks][e], s[kt], 0, 0, 0);
-            } else {
-              s[kt] = PromptMma<T>::mul(kf[kt][ks], qf[ks], s[kt]);
+            for (int i = 0; i < KS; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
           }
-        if constexpr (!F32) {
-          // half of the fragments ahead of the first product, then one read behind each product
-          __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        constexpr int HALVES = KT / 32;
+        if (more) issue(t + KG, buf ^ 1, kt * RP / HALVES, (kt + 1) * RP / HALVES);
       }
+      if (t + 2 * KG < t1) get_ids(t + 2 * KG);
       if (key0 + KT > full_hi || key0 < full_lo || missing) {
         unsigned long long there = ~0ull;
         if (PAGED && missing) {
@@ -428,6 +443,9 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
           }
         }
       }
+    } else {
+      if (more) issue(t + KG, buf ^ 1, 0, RP);
+      if (t + 2 * KG < t1) get_ids(t + 2 * KG);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -520,7 +538,7 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
       if constexpr (PAGED) {
         const int page = lookup(t);
         there = page_ok(page);
-        return paged_row(base, page, t);
+        return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + paged_offset(page, t));
       } else {
         there = true;
         return base + t * stride;
@@ -638,6 +656,9 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
     if (d->pages->type != d->type) return KX_EUNSUPPORTED;
     if (d->pages->kv_head_num != d->kv_head_num || d->pages->head_size != d->head_size || d->pages->batch != d->batch)
       return KX_EINVAL;
+    // (a page's and a row's bytes are counted in 32 bits)
+    if ((uint64_t)d->pages->page_stride * bytes > 0xffffffffull || (uint64_t)d->pages->row_stride * bytes * 16 > 0x7fffffffull)
+      return KX_EUNSUPPORTED;
     a.kv = paged_view(*d->pages);
     a.k = a.kv.key;
     a.v = a.kv.value;
