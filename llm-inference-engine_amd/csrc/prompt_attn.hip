@@ -71,7 +71,8 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
   const int lane = lane_id();
   int done = 0;
   for (int base = 0; base < a.batch; base += 64) {
-    int b = base + lane, q0 = 0, n = 0, k0 = 0, keys = 0;
+    const int b = base + lane;
+    int q0 = 0, n = 0, k0 = 0, keys = 0;
     if (b < a.batch) {
       q0 = clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b), a.q_rows);
       n = max(clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b + 1), a.q_rows) - q0, 0);
@@ -84,6 +85,8 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
     }
     // The sequences (64 at a time) in falling order of their keys, each one's last blocks first: long chains of tiles
     // start early.  (Six pieces of 118 .. 1024 rows over 425 .. 4298 keys: 178 us in index order, 146 so, one group.)
+    const int mine = (int)(((int64_t)n * a.kv_mul + ROWS - 1) / ROWS);
+    int blocks = mine, from = lane;
     if (a.batch > 1) {
       int place = 0;
       for (int j = 0; j < min(a.batch - base, 64); ++j) {
@@ -91,24 +94,19 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
         place += other > keys || (other == keys && j < lane);
       }
       if (b >= a.batch) place = lane;
-      const int from = __builtin_amdgcn_ds_permute(place << 2, lane) << 2;
-      b = base + (from >> 2);
-      q0 = __builtin_amdgcn_ds_bpermute(from, q0);
-      n = __builtin_amdgcn_ds_bpermute(from, n);
-      k0 = __builtin_amdgcn_ds_bpermute(from, k0);
-      keys = __builtin_amdgcn_ds_bpermute(from, keys);
+      from = __builtin_amdgcn_ds_permute(place << 2, lane);
+      blocks = __builtin_amdgcn_ds_permute(place << 2, mine);
     }
-    const int blocks = (int)(((int64_t)n * a.kv_mul + ROWS - 1) / ROWS);
     const int upto = wave_scan(blocks);
     const unsigned long long past = __ballot(done + upto > item);
     if (past) {
-      const int l = __builtin_ctzll(past);
-      w.b = __builtin_amdgcn_readlane(b, l);
+      const int at = __builtin_ctzll(past), l = __builtin_amdgcn_readlane(from, at);
+      w.b = base + l;
       w.q0 = __builtin_amdgcn_readlane(q0, l);
       w.n = __builtin_amdgcn_readlane(n, l);
       w.k0 = __builtin_amdgcn_readlane(k0, l);
       w.keys = __builtin_amdgcn_readlane(keys, l);
-      w.block = done + __builtin_amdgcn_readlane(upto, l) - 1 - item;
+      w.block = done + __builtin_amdgcn_readlane(upto, at) - 1 - item;
       return true;
     }
     done += __builtin_amdgcn_readlane(upto, 63);
@@ -171,6 +169,7 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
   constexpr float kShift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
   constexpr int KS = HS * (int)sizeof(T) / 32;   // 32-byte steps of the first product
   static_assert(KP * KG % NW == 0 || KP * KG < NW, "");
+  __shared__ int sm_missing[PAGED ? NW : 1];
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers of KG tiles, K and V each
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef const __attribute__((address_space(3))) char* lds_bytes;
@@ -210,6 +209,18 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
     return (uint64_t)(page_ok(page) ? (unsigned)page : 0u) * page_bytes +
            (uint64_t)(unsigned)(t - a.kv.div.page(t) * a.kv.div.size) * row_bytes;
   };
+  // ---- queries: lane (pair, half) holds the pieces of its row that meet its pieces of a K row ----
+  typedef typename PromptMma<T>::frag frag;
+  frag qf[KS];
+  const T* qrow = reinterpret_cast<const T*>(a.q) + (w.q0 + my_row) * a.q_stride + (kvh * a.kv_mul + my_head) * HS;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    qf[ks] = *KX_CK(a, PP_Q, reinterpret_cast<const frag*>(reinterpret_cast<const char*>(qrow) + 32 * ks + 16 * half));
+  // A page that is not there is looked for once, beside the first tiles' way here, and tile by tile only if there is one.
+  const int last_col = PAGED && t0 < t1 ? a.kv.div.page(hi - 1) : 0, col = PAGED ? a.kv.div.page(lo) + (int)threadIdx.x : 0;
+  int probe = 0;
+  if (PAGED && t0 < t1) probe = *KX_CK(a, PP_TABLE, table + min(col, last_col));
+
   // The KG tiles of a buffer are consecutive, so its K rows are KG * KT consecutive keys.  DMA pair j of a wave, one
   // instruction for K and one for V: the first of its rows among the keys, and a lane's.
   auto pair_first = [&](int j) { return (wave + NW * j) * RPP; };
@@ -283,23 +294,6 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
     issue(t0, 0, 0, RP);
     if (t0 + KG < t1) get_ids(t0 + KG);
   }
-  // a page that is not there: looked for once, and tile by tile only if there is one
-  bool missing = false;
-  if constexpr (PAGED) {
-    if (t0 < t1) {
-      const int c1 = a.kv.div.page(hi - 1);
-      for (int c = a.kv.div.page(lo) + (int)threadIdx.x; c <= c1; c += NW * 64) missing |= !page_ok(*KX_CK(a, PP_TABLE, table + c));
-    }
-    missing = __syncthreads_or(missing);
-  }
-
-  // ---- queries: lane (pair, half) holds the pieces of its row that meet its pieces of a K row ----
-  typedef typename PromptMma<T>::frag frag;
-  frag qf[KS];
-  const T* qrow = reinterpret_cast<const T*>(a.q) + (w.q0 + my_row) * a.q_stride + (kvh * a.kv_mul + my_head) * HS;
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-    qf[ks] = *KX_CK(a, PP_Q, reinterpret_cast<const frag*>(reinterpret_cast<const char*>(qrow) + 32 * ks + 16 * half));
   // scores in powers of two; a negative scale turns the queries' sign, and a scale of zero still hides (-inf * 0 is NaN)
   if (a.scale < 0.f) {
 #pragma unroll
@@ -329,8 +323,21 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
   float m = -INFINITY, l = 0.f;  // m in units of the raw product
 
+  bool missing = false;
+  if (PAGED && t0 < t1) {
+    missing = !page_ok(probe);
+    for (int at = col + NW * 64; at <= last_col; at += NW * 64) missing |= !page_ok(*KX_CK(a, PP_TABLE, table + at));
+    const bool any = __ballot(missing) != 0;
+    if (lane == 0) sm_missing[wave] = any;
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  if (PAGED && t0 < t1) {
+    missing = false;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) missing |= sm_missing[v] != 0;
+    missing = __builtin_amdgcn_readfirstlane(missing);
+  }
   for (int t = t0, buf = 0; t < t1; t += KG, buf ^= 1) {
     // The next tiles are requested in two parts beside the scores: the LDS-DMA of a CU takes 64 bytes a cycle, and a wave
     // that sends all of its share at once waits for that.
