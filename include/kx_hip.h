@@ -595,11 +595,11 @@ enum { KX_F32 = 0, KX_F16 = 1, KX_BF16 = 2 };
  * Position t of sequence b is row t % page_size of page table[b * table_stride + t / page_size].
  * table and seq_lens are device memory, read by the kernels: a captured launch is replayed as they
  * change.  seq_lens[b] counts the rows of sequence b INCLUDING those of the call; a length below zero
- * counts as zero, one above table_pages * page_size as that.  A table entry outside 0..num_pages-1 is
- * a page that is not there (one that a sliding window has left behind, say): nothing is read or
- * written through it and its positions are seen by no query.
+ * counts as zero.  A table entry outside 0..num_pages-1 is a page that is not there (one that a sliding
+ * window has left behind, say): nothing is read or written through it and its positions are seen by no
+ * query.  So are positions from table_pages * page_size on, where a length goes past that.
  * head_size 32, 64 or 128 (else KX_EUNSUPPORTED); any page size; strides that are at least head_size and
- * multiples of 16 bytes, key and value aligned to 16 bytes; page_size * table_pages below 2^31. */
+ * multiples of 16 bytes, key and value aligned to 16 bytes; page_size * table_pages at most 2^31 - 256. */
 typedef struct kx_paged_kv {
   int32_t type;          /* KX_F32 / KX_F16 / KX_BF16 */
   int32_t kv_head_num, head_size;
@@ -625,7 +625,8 @@ typedef struct kx_paged_kv {
  * is outside 0 .. table_pages * page_size - 1, has no page or (when rotating) lies past table_rows is not filed; past
  * table_rows or below zero its q row is left alone too.  Rows of no sequence (below cu_rows[0], from cu_rows[batch] on) are left
  * alone.  No two rows of a call may have the same place in the pages.  Strides in elements, at least the
- * row's width and multiples of 16 bytes; pointers aligned to 16 bytes (KX_EINVAL). */
+ * row's width and multiples of 16 bytes, q's and q_out's the same where they are one; pointers aligned to 16 bytes (KX_EINVAL).
+ * KX_ELIMIT from 2^25 rows on, or for 2^30 elements of q, k and v in a row. */
 typedef struct kx_paged_write_desc {
   kx_paged_kv kv;
   int32_t src_type;
@@ -655,8 +656,10 @@ int kx_paged_write(const kx_paged_write_desc* desc, void* stream);
  * a cache of the same type.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
  * must be ZERO before its first use and is left ready for the next call by every call; calls that
  * share one must not overlap in time (kx_attn_workspace_reset's rule: after an aborted launch clear it again).
+ * One workspace may serve calls of any sizes and those of kx_token_logprobs, but of no other entry.  scale is finite.
  * The lengths are read by the kernel, which cuts the batch's keys evenly over the chip.  KX_EUNSUPPORTED for more
- * than 1024 kv heads (a kv head of more than 16 query heads counts once per 16). */
+ * than 1024 kv heads (a kv head of more than 16 query heads counts once per 16), KX_ELIMIT where
+ * batch * kv heads pass 2^24. */
 typedef struct kx_paged_decode_desc {
   kx_paged_kv kv;
   int32_t q_type;
@@ -681,7 +684,10 @@ int kx_paged_decode(const kx_paged_decode_desc* desc, void* stream);
  * A row that sees nothing gets zeros; rows of no sequence are left alone.  All of one type
  * (KX_F16 / KX_BF16: matrix-core products of that type with fp32 sums and softmax, probabilities
  * rounded to it for the second product; KX_F32: fp32 throughout).  head_size 32, 64 or 128.  Strides in elements (q and
- * out: head_num * head_size or more, k and v: kv_head_num * head_size or more), multiples of 16 bytes. */
+ * out: head_num * head_size or more, k and v: kv_head_num * head_size or more), multiples of 16 bytes; pointers aligned
+ * to 16 bytes; scale finite.  KX_EUNSUPPORTED for packed k or v rows 8 MiB or more apart, pages 4 GiB or more
+ * apart or rows of a page 128 MiB or more apart; KX_ELIMIT for 2^31 - 65536 pairs of a row and a head of one kv head, 2^31 - 256
+ * key rows, or more than 2^23 workgroups (a workgroup has 64 such pairs or more, a sequence one workgroup per kv head or more). */
 typedef struct kx_prompt_attn_desc {
   int32_t type;
   int32_t head_num, kv_head_num, head_size;
@@ -711,7 +717,8 @@ int kx_prompt_attention(const kx_prompt_attn_desc* desc, void* stream);
  * in fp32.  A token below zero is none: logprob 0; one past the vocabulary: NaN.  A row that is no
  * distribution (holds NaN or +inf, or nothing but -inf) gives NaN for the three kinds of numbers, and its ids in order.
  * Logits of `type`, rows at row_stride elements (any, >= vocab), aligned to their element.  workspace as for
- * kx_paged_decode, of kx_token_logprobs_workspace_bytes(rows, vocab, top_n) bytes. */
+ * kx_paged_decode, of kx_token_logprobs_workspace_bytes(rows, vocab, top_n) bytes.  KX_ELIMIT from 2^24 rows or 2^31 - 256
+ * logits in a row on. */
 #define KX_LOGPROBS_TOP_MAX 32
 typedef struct kx_logprobs_desc {
   int32_t type;

@@ -32,7 +32,7 @@ constexpr int kLpList = 512;      // elements that are ranked at once
 constexpr int kLpMaxParts = 32;   // of a row
 constexpr int kLpSlots = 1024;    // workgroups that few rows are cut for
 constexpr int kLpRecord = 16 + 8 * KX_LOGPROBS_TOP_MAX;  // bytes: m, z, s, -, then the list
-constexpr size_t kLpTicketBytes = (size_t)kLpSlots * 64;
+static_assert(kLpSlots * kTicketStride <= kTicketBytes, "");
 
 struct LogprobsArgs {
   const void* logits;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     __syncthreads();
     if (tid == 0) {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-      sm_last = atomicInc(KX_CK(a, PL_WS, a.tickets + row * 16), (unsigned)a.parts - 1u) == (unsigned)a.parts - 1u;  // wraps to 0
+      sm_last = atomicInc(KX_CK(a, PL_WS, a.tickets + row * (kTicketStride / 4)), (unsigned)a.parts - 1u) == (unsigned)a.parts - 1u;  // wraps to 0
     }
     __syncthreads();
     if (!sm_last) return;
@@ -389,7 +389,7 @@ static int logprobs_parts(int rows, int vocab, int kind) {
 extern "C" size_t kx_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_n) {
   using namespace kx;
   if (rows <= 0 || vocab <= 0 || top_n < 0) return 0;
-  return kLpTicketBytes + (size_t)kLpSlots * kLpRecord;  // the tickets' place is the same for every call
+  return kTicketBytes + (size_t)kLpSlots * kLpRecord;
 }
 
 extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
@@ -403,6 +403,7 @@ extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
   if (d->top_n > 0 && (!d->top_ids || !d->top_logprobs)) return KX_EINVAL;
   if (!d->workspace || d->workspace_bytes < kx_token_logprobs_workspace_bytes(d->rows, d->vocab, d->top_n)) return KX_EWORKSPACE;
   if ((uintptr_t)d->workspace % 256) return KX_EINVAL;
+  if (!grid_fits(d->rows, kLpThreads) || d->vocab > kMostPositions) return KX_ELIMIT;
   LogprobsArgs a{};
   a.logits = d->logits;
   a.tokens = d->tokens;
@@ -411,7 +412,7 @@ extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
   a.top_ids = d->top_ids;
   a.top_logprobs = d->top_logprobs;
   a.tickets = static_cast<unsigned*>(d->workspace);
-  a.records = static_cast<char*>(d->workspace) + kLpTicketBytes;
+  a.records = static_cast<char*>(d->workspace) + kTicketBytes;
   a.row_stride = d->row_stride;
   a.rows = d->rows;
   a.vocab = d->vocab;

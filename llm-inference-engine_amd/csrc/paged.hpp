@@ -20,7 +20,7 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive prefix sum over 
   return v;
 }
 
-// Four / eight consecutive elements, widened exactly.
+// Four consecutive elements, widened exactly.
 __device__ __forceinline__ void load4(const float* p, float (&o)[4]) {
   const f32x4 v = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
@@ -42,15 +42,6 @@ template <typename T> __device__ __forceinline__ T round_to(float x);
 template <> __device__ __forceinline__ float round_to<float>(float x) { return x; }
 template <> __device__ __forceinline__ _Float16 round_to<_Float16>(float x) { return x != x ? (_Float16)x : sat_f16(x); }
 template <> __device__ __forceinline__ __bf16 round_to<__bf16>(float x) { return (__bf16)x; }
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
-  typedef T vec __attribute__((ext_vector_type(4)));
-  vec o;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = round_to<T>(v[i]);
-  *reinterpret_cast<vec*>(p) = o;
-}
 
 // Division of a position by the page size: n / d = (2n * mul) >> (32 + shift) for n < 2^31, with
 // 2^shift >= d and mul = ceil(2^(31 + shift) / d) (the rounded-up reciprocal is off by less than one part in
@@ -82,6 +73,14 @@ inline PagedView paged_view(const kx_paged_kv& d) {
                    d.page_stride, d.row_stride, d.head_stride, d.table_stride,
                    page_div(d.page_size), d.num_pages, d.table_pages, d.batch};
 }
+// Positions of a sequence, and elements of a row of logits: the end of a last tile or step still fits 31 bits.
+constexpr int64_t kMostPositions = 0x7fffff00ll;
+// The tickets of the workgroups that meet in a workspace (64 bytes each) lie ahead of all records, at the same place for
+// every call of every entry, whatever its sizes: no call's records ever lie where another's tickets are, so calls of
+// different sizes and kinds can follow each other in one workspace.
+constexpr size_t kTicketStride = 64, kTicketBytes = 3 * 1024 * kTicketStride;
+// a launch has fewer than 2^32 threads
+inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffll; }
 inline size_t kind_bytes(int32_t kind) { return kind == KX_F32 ? 4 : 2; }
 inline bool kind_known(int32_t kind) { return kind == KX_F32 || kind == KX_F16 || kind == KX_BF16; }
 inline bool head_size_known(int32_t hs) { return hs == 32 || hs == 64 || hs == 128; }
@@ -101,7 +100,7 @@ inline int paged_check(const kx_paged_kv& d) {
   if (!stride_ok(d.page_stride, d.head_size, unit) || !stride_ok(d.row_stride, d.head_size, unit) ||
       !stride_ok(d.head_stride, d.head_size, unit) || d.table_stride < d.table_pages)
     return KX_EINVAL;
-  if ((int64_t)d.page_size * d.table_pages > 0x7fffffffll) return KX_EINVAL;
+  if ((int64_t)d.page_size * d.table_pages > kMostPositions) return KX_EINVAL;
   return KX_OK;
 }
 // queries of a type over a cache of a type: fp32 over any, 16-bit ones over their own

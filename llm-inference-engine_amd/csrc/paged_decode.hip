@@ -34,7 +34,6 @@ constexpr int kPdWaves = 4;
 constexpr int kPdSlots = 1024;      // workgroups that a batch is cut for
 constexpr int kPdMaxSplits = 128;   // chunks of one sequence
 constexpr int kPdLeastChunk = 16;   // tiles of a chunk at least (16 fp32 sequences of 500-4400 keys: 33.2 us with 8, 29.3 with 16)
-constexpr size_t kPdTicketStride = 64;
 
 struct PagedDecodeArgs {
   PagedView kv;
@@ -58,13 +57,12 @@ struct DecodeWork {
 template <int TK>
 __device__ __forceinline__ bool find_work(const PagedDecodeArgs& a, int item, DecodeWork& w) {
   const int lane = lane_id(), batch = a.kv.batch;
-  auto length = [&](int b) {
-    return b < batch ? min(max(*KX_CK(a, PD_LENS, a.kv.seq_lens + b), 0), a.kv.capacity()) : 0;
-  };
+  auto length = [&](int b) { return b < batch ? max(*KX_CK(a, PD_LENS, a.kv.seq_lens + b), 0) : 0; };
   auto first = [&](int len) { return a.window > 0 ? max(0, len - a.window) : 0; };
-  auto tiles_of = [&](int len) { return len > 0 ? (len - 1) / TK - first(len) / TK + 1 : 0; };
+  auto rows = [&](int len) { return min(len, a.kv.capacity()); };  // those that the table has places for
+  auto tiles_of = [&](int len) { return rows(len) > first(len) ? (rows(len) - 1) / TK - first(len) / TK + 1 : 0; };
   // The chunk length: an even share, and no sequence in more than kPdMaxSplits.  (Sums past 2^24 tiles are rounded:
-  // the grid and the records have one item to spare for the share, the limit gets one tile more.)
+  // the grid and the records have one item to spare for the share, the limit gets one tile more.  2^27 tiles hold any sequence.)
   float sum = 0.f, most = 0.f;
   int len = 0, tiles = 0;
   for (int base = 0; base < batch; base += 64) {
@@ -76,7 +74,7 @@ __device__ __forceinline__ bool find_work(const PagedDecodeArgs& a, int item, De
   sum = wave_sum(sum);
   most = wave_max(most);
   const float share = ceilf(sum / (float)a.items), limit = ceilf(most / (float)kPdMaxSplits) + (most >= 16777216.f ? 1.f : 0.f);
-  const int chunk = max(kPdLeastChunk, ((int)fmaxf(share, limit) + kPdWaves - 1) / kPdWaves * kPdWaves);
+  const int chunk = max(kPdLeastChunk, ((int)fminf(fmaxf(share, limit), 134217728.f) + kPdWaves - 1) / kPdWaves * kPdWaves);
   int done = 0, records = 0;
   for (int base = 0; base < batch; base += 64) {
     if (batch > 64) {
@@ -89,11 +87,12 @@ __device__ __forceinline__ bool find_work(const PagedDecodeArgs& a, int item, De
     if (past) {
       const int l = __builtin_ctzll(past);
       w.b = base + l;
-      w.len = __builtin_amdgcn_readlane(len, l);
+      const int length_b = __builtin_amdgcn_readlane(len, l);
+      w.len = rows(length_b);
       w.nsplit = __builtin_amdgcn_readlane(n, l);
       w.split = item - (done + __builtin_amdgcn_readlane(upto, l) - w.nsplit);
       w.record = records + __builtin_amdgcn_readlane(cut, l) - w.nsplit;
-      w.lo = first(w.len);
+      w.lo = first(length_b);
       const int all = __builtin_amdgcn_readlane(tiles, l);
       const int each = all / w.nsplit, more = all % w.nsplit;
       w.tile0 = w.lo / TK + w.split * each + min(w.split, more);
@@ -478,7 +477,7 @@ __global__ __launch_bounds__(kPdWaves * 64, 2) void paged_decode_kernel(const Pa
   __syncthreads();
   if (threadIdx.x == 0) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    unsigned* ticket = a.tickets + ((int64_t)w.record * heads_of + hv) * (kPdTicketStride / 4);
+    unsigned* ticket = a.tickets + ((int64_t)w.record * heads_of + hv) * (kTicketStride / 4);
     sm_last = atomicInc(KX_CK(a, PD_WS, ticket), (unsigned)w.nsplit - 1u) == (unsigned)w.nsplit - 1u;  // wraps to 0
   }
   __syncthreads();
@@ -555,9 +554,8 @@ static int decode_items(int kv_heads, int groups) {
 // Records that a call may use.  A sequence that is cut has more tiles than a chunk, so its chunks are fewer than twice
 // its share of `items`; one more for the rounding of the share.
 static int decode_records(int items) { return 2 * items + 1; }
-// The tickets' place is the same for every call, whatever its batch and heads: no call's records ever lie there.
 // records * (kv heads * groups) <= 2 * slots + kv heads * groups, and those are kPdSlots at most.
-constexpr size_t kPdTicketBytes = 3 * kPdSlots * kPdTicketStride;
+static_assert(3 * kPdSlots * kTicketStride <= kTicketBytes, "");
 
 template <typename QT, typename KVT, int HS>
 static void paged_decode_launch(const PagedDecodeArgs& a, hipStream_t s) {
@@ -580,7 +578,7 @@ extern "C" size_t kx_paged_decode_workspace_bytes(int32_t batch, int32_t head_nu
   using namespace kx;
   if (batch <= 0 || head_num <= 0 || kv_head_num <= 0 || head_num % kv_head_num || head_size <= 0) return 0;
   const DecodeHeads h = decode_heads(head_num, kv_head_num);
-  return kPdTicketBytes + (size_t)decode_records(decode_items(kv_head_num, h.groups)) * kv_head_num * h.groups *
+  return kTicketBytes + (size_t)decode_records(decode_items(kv_head_num, h.groups)) * kv_head_num * h.groups *
                               h.group_heads * (head_size + 4) * sizeof(float);
 }
 
@@ -589,7 +587,8 @@ extern "C" int kx_paged_decode(const kx_paged_decode_desc* d, void* stream) {
   if (!d || d->kv.batch < 0) return KX_EINVAL;
   if (d->kv.batch == 0) return KX_OK;
   if (const int rc = paged_check(d->kv)) return rc;
-  if (!kind_known(d->q_type) || d->head_num <= 0 || d->head_num % d->kv.kv_head_num || d->window < 0) return KX_EINVAL;
+  if (!kind_known(d->q_type) || d->head_num <= 0 || d->head_num % d->kv.kv_head_num || d->window < 0 || !isfinite(d->scale))
+    return KX_EINVAL;
   if (!kinds_fit(d->q_type, d->kv.type)) return KX_EUNSUPPORTED;
   const int64_t q_dim = (int64_t)d->head_num * d->kv.head_size;
   const size_t unit = 16 / kind_bytes(d->q_type);
@@ -605,7 +604,7 @@ extern "C" int kx_paged_decode(const kx_paged_decode_desc* d, void* stream) {
   a.q = d->q;
   a.out = d->out;
   a.tickets = static_cast<unsigned*>(d->workspace);
-  a.records = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kPdTicketBytes);
+  a.records = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kTicketBytes);
   a.q_stride = d->q_stride;
   a.out_stride = d->out_stride;
   a.head_num = d->head_num;
@@ -617,7 +616,7 @@ extern "C" int kx_paged_decode(const kx_paged_decode_desc* d, void* stream) {
   if ((int64_t)a.kv_heads * a.groups > kPdSlots) return KX_EUNSUPPORTED;
   a.items = decode_items(a.kv_heads, a.groups);
   a.scale = d->scale;
-  if ((int64_t)(a.items + a.kv.batch + 1) * a.kv_heads * a.groups > 0x7fffffffll) return KX_ELIMIT;
+  if (!grid_fits(((int64_t)a.items + a.kv.batch + 1) * a.kv_heads * a.groups, kPdWaves * 64)) return KX_ELIMIT;
   const void* operands[] = {a.kv.key, a.kv.value, a.kv.table, a.kv.seq_lens, a.q, a.out, d->workspace};
   for (int i = 0; i < 7; ++i) KX_BSET(a, i, operands[i]);
   (void)operands;

@@ -97,11 +97,11 @@ __global__ __launch_bounds__(128) void paged_write_kernel(const PagedWriteArgs a
 
   const int b = __builtin_amdgcn_readfirstlane(sequence_of_row(a, row));
   if (b < 0) return;
-  const int len = min(max(*KX_CK(a, PW_LENS, a.kv.seq_lens + b), 0), a.kv.capacity());
-  const int64_t at = (int64_t)row - *KX_CK(a, PW_CU, a.cu + b + 1) + len;
-  if (at < 0 || at >= len || (a.sin_cache && at >= a.table_rows)) return;
+  const int64_t at = (int64_t)row - *KX_CK(a, PW_CU, a.cu + b + 1) + *KX_CK(a, PW_LENS, a.kv.seq_lens + b);  // below the length
+  if (at < 0 || (a.sin_cache && at >= a.table_rows)) return;
   const int pos = (int)at, page_col = a.kv.div.page(pos);
-  const int page = *KX_CK(a, PW_TABLE, a.kv.table + (b * a.kv.table_stride + page_col));
+  int page = -1;
+  if (pos < a.kv.capacity()) page = *KX_CK(a, PW_TABLE, a.kv.table + (b * a.kv.table_stride + page_col));
   const bool filed = page >= 0 && page < a.kv.num_pages;
   const int64_t slot = page * a.kv.page_stride + (pos - page_col * a.kv.div.size) * a.kv.row_stride;
   float sn[V], cs[V];
@@ -188,6 +188,8 @@ extern "C" int kx_paged_write(const kx_paged_write_desc* d, void* stream) {
   if (!stride_ok(d->k_stride, kv_dim, unit) || !stride_ok(d->v_stride, kv_dim, unit)) return KX_EINVAL;
   if (d->q && (!stride_ok(d->q_stride, q_dim, unit) || !stride_ok(d->q_out_stride, q_dim, unit))) return KX_EINVAL;
   if (!aligned16(d->k) || !aligned16(d->v) || !aligned16(d->q) || !aligned16(d->q_out)) return KX_EINVAL;
+  if (d->q && d->q == d->q_out && d->q_stride != d->q_out_stride) return KX_EINVAL;  // one row's results over another's elements
+  if (!grid_fits(d->rows, 128) || (d->q ? q_dim : 0) + 2 * kv_dim > 0x3fffffff) return KX_ELIMIT;
   PagedWriteArgs a{};
   a.kv = paged_view(d->kv);
   a.key = static_cast<char*>(d->kv.key);

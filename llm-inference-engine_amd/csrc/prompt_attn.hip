@@ -61,6 +61,7 @@ struct PromptArgs {
 struct PromptWork {
   int b, q0, n;      // sequence, its first row in q, its rows
   int k0, keys;      // first key row (packed), keys
+  int p0;            // position of the first row, below zero with fewer keys than rows
   int block;         // 32 * waves pairs from here
 };
 
@@ -72,15 +73,16 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
   int done = 0;
   for (int base = 0; base < a.batch; base += 64) {
     const int b = base + lane;
-    int q0 = 0, n = 0, k0 = 0, keys = 0;
+    int q0 = 0, n = 0, k0 = 0, keys = 0, length = 0;
     if (b < a.batch) {
       q0 = clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b), a.q_rows);
       n = max(clamp_row(*KX_CK(a, PP_CUQ, a.cu_q + b + 1), a.q_rows) - q0, 0);
       if (PAGED) {
-        keys = min(max(*KX_CK(a, PP_LENS, a.kv.seq_lens + b), 0), a.kv.capacity());
+        length = max(*KX_CK(a, PP_LENS, a.kv.seq_lens + b), 0);
+        keys = min(length, a.kv.capacity());
       } else {
         k0 = clamp_row(*KX_CK(a, PP_CUK, a.cu_k + b), a.k_rows);
-        keys = max(clamp_row(*KX_CK(a, PP_CUK, a.cu_k + b + 1), a.k_rows) - k0, 0);
+        length = keys = max(clamp_row(*KX_CK(a, PP_CUK, a.cu_k + b + 1), a.k_rows) - k0, 0);
       }
     }
     // The sequences (64 at a time) in falling order of their keys, each one's last blocks first: long chains of tiles
@@ -106,6 +108,7 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
       w.n = __builtin_amdgcn_readlane(n, l);
       w.k0 = __builtin_amdgcn_readlane(k0, l);
       w.keys = __builtin_amdgcn_readlane(keys, l);
+      w.p0 = __builtin_amdgcn_readlane(length, l) - w.n;
       w.block = done + __builtin_amdgcn_readlane(upto, at) - 1 - item;
       return true;
     }
@@ -183,9 +186,8 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
 
   // ---- this workgroup's and this wave's pairs, and what they see ----
   const int pairs = w.n * a.kv_mul, f0 = w.block * PAIRS;
-  const int p0 = w.keys - w.n;  // position of row 0, below zero with fewer keys than rows
-  auto hi_of = [&](int row) { return a.causal ? max(min(p0 + row + 1, w.keys), 0) : w.keys; };
-  auto lo_of = [&](int row) { return a.window > 0 ? max(p0 + row - a.window + 1, 0) : 0; };
+  auto hi_of = [&](int row) { return a.causal ? max(min(w.p0 + row + 1, w.keys), 0) : w.keys; };
+  auto lo_of = [&](int row) { return a.window > 0 ? max(max(w.p0 + row, 0) - a.window + 1, 0) : 0; };
   auto row_of = [&](int f) { return a.mul_div.page(min(f, pairs - 1)); };
   const int hi = hi_of(row_of(f0 + PAIRS - 1)), lo = min(lo_of(row_of(f0)), hi);
   const int t0 = lo / KT, t1 = hi > lo ? (hi + KT - 1) / KT : t0;
@@ -603,12 +605,12 @@ constexpr int prompt_lds() {
 template <typename T, int HS, int MODE, int KG>
 static int prompt_launch(const PromptArgs& a, hipStream_t s) {
   constexpr int pairs = kPaWaves / KG * 32, lds = prompt_lds<T, HS, KG>();
+  // blocks of the sequences: an even share of all pairs and one more each
+  const int64_t items = (int64_t)a.q_rows * a.kv_mul / pairs + a.batch;
+  if (!grid_fits(items * a.kv_heads, kPaWaves * 64)) return KX_ELIMIT;
   static OncePerDevice limit;
   if (lds > 32768)
     if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, KG>), lds)) return rc;
-  // blocks of the sequences: an even share of all pairs and one more each
-  const int64_t items = (int64_t)a.q_rows * a.kv_mul / pairs + a.batch;
-  if (items * a.kv_heads > 0x7fffffffll) return KX_ELIMIT;
   hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, KG>), dim3((unsigned)(items * a.kv_heads)), dim3(kPaWaves * 64), lds, s, a);
   KX_LAUNCH_CHECK();
   return KX_OK;
@@ -650,7 +652,7 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
   if (d->batch == 0 || d->q_rows == 0) return KX_OK;
   if (!kind_known(d->type) || d->head_num <= 0 || d->kv_head_num <= 0 || d->head_num % d->kv_head_num) return KX_EINVAL;
   if (!head_size_known(d->head_size)) return KX_EUNSUPPORTED;
-  if (d->window < 0 || (d->window > 0 && !d->causal)) return KX_EINVAL;
+  if (d->window < 0 || (d->window > 0 && !d->causal) || !isfinite(d->scale)) return KX_EINVAL;
   const int64_t q_dim = (int64_t)d->head_num * d->head_size, kv_dim = (int64_t)d->kv_head_num * d->head_size;
   const size_t bytes = kind_bytes(d->type), unit = 16 / bytes;
   if (!d->q || !d->out || !d->cu_q || (uintptr_t)d->cu_q % 4 || !aligned16(d->q) || !aligned16(d->out) ||
@@ -680,7 +682,8 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
     a.v = static_cast<const char*>(d->v);
   }
   const int32_t kv_mul = d->head_num / d->kv_head_num;
-  if ((int64_t)d->q_rows * kv_mul > 0x7fff0000ll) return KX_ELIMIT;  // (row, head) pairs are counted in 31 bits
+  // (row, head) pairs, keys and the elements of a row are counted in 31 bits
+  if ((int64_t)d->q_rows * kv_mul > 0x7fff0000ll || (!d->pages && d->k_rows > kMostPositions) || q_dim > 0x7fffffffll) return KX_ELIMIT;
   a.q = static_cast<const char*>(d->q); a.out = static_cast<char*>(d->out); a.cu_q = d->cu_q; a.cu_k = d->cu_k;
   a.q_stride = d->q_stride; a.k_stride = d->k_stride; a.v_stride = d->v_stride; a.out_stride = d->out_stride;
   a.batch = d->batch; a.kv_heads = d->kv_head_num; a.kv_mul = kv_mul; a.mul_div = page_div(kv_mul);

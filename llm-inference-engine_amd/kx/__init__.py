@@ -655,6 +655,8 @@ def paged_write(pool, table, seq_lens, cu_rows, k, v, q=None, rope=None, variant
     (sin, cos) tables [positions][hs] or None.  Returns the rotated q as fp32 (None without q)."""
     tb, sl, cu = (Buf.from_numpy(np.asarray(a, np.int32)) for a in (table, seq_lens, cu_rows))
     rows, heads = k.shape[0], 0 if q is None else q.shape[1]
+    assert k.shape == v.shape == (rows, *pool.shape[2:]) and (q is None or q.shape[::2] == k.shape[::2])
+    assert len(seq_lens) == len(table) == len(cu_rows) - 1 and (rope is None or rope[0].shape == rope[1].shape == (len(rope[0]), k.shape[2]))
     dk, dv = Buf.from_numpy(to_kind(k, src_kind)), Buf.from_numpy(to_kind(v, src_kind))
     d = PagedWriteDesc(kv=pool.desc(tb, sl), src_type=src_kind, rows=rows, head_num=heads, rope_variant=variant,
                        cu_rows=cu.ptr, k=dk.ptr, k_stride=k.shape[1] * k.shape[2], v=dv.ptr,
@@ -676,6 +678,7 @@ def paged_decode(pool, table, seq_lens, q, scale=None, window=0, q_kind=F32, wor
     """kx_paged_decode: q [batch][heads][hs] fp32 (rounded to q_kind); returns [batch][heads][hs] as fp32.
     workspace: a zero-filled Buf that earlier calls may have used."""
     batch, heads, hs = q.shape
+    assert len(table) == len(seq_lens) == batch and hs == pool.shape[3]
     tb, sl = (Buf.from_numpy(np.asarray(a, np.int32)) for a in (table, seq_lens))
     dq, out = Buf.from_numpy(to_kind(q, q_kind)), Buf.zeros(q.shape, KIND_DTYPE[q_kind])
     if workspace is None:
@@ -694,6 +697,10 @@ def prompt_attention(q, cu_q, k=None, v=None, cu_k=None, pool=None, table=None, 
     lengths; q [rows][heads][hs].  fp32 arrays, rounded to `kind`; returns [rows][heads][hs] as fp32.  fill: what
     the output holds before the call."""
     rows, heads, hs = q.shape
+    if pool is None:
+        assert k.shape == v.shape and k.shape[2] == hs and (cu_k is None or len(cu_k) == len(cu_q))
+    else:
+        assert len(table) == len(seq_lens) == len(cu_q) - 1 and hs == pool.shape[3]
     cu = Buf.from_numpy(np.asarray(cu_q, np.int32))
     dq, out = Buf.from_numpy(to_kind(q, kind)), Buf.from_numpy(to_kind(np.full(q.shape, fill), kind))
     d = PromptAttnDesc(type=kind, head_num=heads, head_size=hs, batch=len(cu_q) - 1, q_rows=rows,
@@ -717,6 +724,7 @@ def token_logprobs(logits, tokens=None, top_n=0, kind=F32, entropy=True, row_str
     """kx_token_logprobs: logits [rows][vocab] fp32 (rounded to `kind`).  Returns (logprob or None, entropy or
     None, top_ids, top_logprobs), the last two [rows][top_n]."""
     rows, vocab = logits.shape
+    assert tokens is None or len(tokens) == rows
     row_stride = row_stride or vocab
     wide = np.zeros((rows, row_stride), np.float32)
     wide[:, :vocab] = logits

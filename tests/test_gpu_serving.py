@@ -17,6 +17,7 @@ import kx  # noqa: E402
 
 U = 2.0 ** -24
 E = {kx.F32: U, kx.F16: 2.0 ** -11, kx.BF16: 2.0 ** -8}
+KINDW = {kx.F32: 4, kx.F16: 2, kx.BF16: 2}
 NAMES = {kx.F32: "f32", kx.F16: "f16", kx.BF16: "bf16"}
 
 
@@ -162,7 +163,7 @@ def test_write_without_rotation_and_saturating():
 
 
 def test_write_leaves_alone_what_has_no_place():
-    """Missing pages, positions below zero, behind the table and behind the sin/cos tables, lengths past the table."""
+    """Missing pages, positions below zero, behind the table of pages and behind the sin/cos tables."""
     rng = np.random.default_rng(6)
     hs, page = 32, 4
     cache = Cache(rng, [12, 12, 12, 12], 1, hs, page, kx.F32, new=[12] * 4)
@@ -178,9 +179,9 @@ def test_write_leaves_alone_what_has_no_place():
     key, value = cache.pool.read()
     want_v = before[1].copy()
     for b in range(4):
-        n, length = new[b], min(lens[b], 12)
+        n = new[b]
         for i in range(n):
-            pos, row = length - n + i, cu[b] + i
+            pos, row = lens[b] - n + i, cu[b] + i
             if 0 <= pos < 10:
                 assert np.abs(got_q[row] - exact_rope(q[row], pos, tables, 1)[0]).max() < 1e-5
                 if 0 <= table[b, pos // page] < 15:
@@ -189,6 +190,37 @@ def test_write_leaves_alone_what_has_no_place():
                 np.testing.assert_array_equal(got_q[row], q[row])
     np.testing.assert_array_equal(value, want_v)
     assert (np.isnan(key) == np.isnan(want_v)).all()
+
+
+def test_lengths_past_the_table():
+    """A sequence that has outgrown its table of pages: what lies in it is filed, read and attended at its own
+    position, the rest is not there."""
+    rng = np.random.default_rng(8)
+    hs, page, window, length, n = 64, 4, 9, 23, 7  # the table holds 20 rows, the new ones are 16 .. 22
+    cache = Cache(rng, [20], 1, hs, page, kx.F32, new=[4])
+    k, v = (rng.standard_normal((n, 1, hs)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((n, 2, hs)).astype(np.float32)
+    before = cache.pool.read()
+    tables = rope_tables(40, hs)
+    got_q = kx.paged_write(cache.pool, cache.table, [length], [0, n], k, v, q, tables, 1)
+    key, value = cache.pool.read()
+    pos = length - n + np.arange(n)
+    assert np.abs(got_q - np.stack([exact_rope(q[i], pos[i], tables, 1)[0] for i in range(n)])).max() < 1e-5
+    last = cache.table[0, 4]
+    np.testing.assert_array_equal(value[last, :, 0], v[:4, 0])
+    others = np.arange(len(key)) != last
+    np.testing.assert_array_equal(value[others], before[1][others])
+    np.testing.assert_array_equal(key[others], before[0][others])
+    ks, vs = (a.reshape(-1, 1, hs)[[t * page + i for t in cache.table[0] for i in range(page)]] for a in (key, value))
+    seen = (np.arange(20)[None] <= pos[:, None]) & (np.arange(20)[None] > pos[:, None] - window)
+    got = kx.prompt_attention(got_q, [0, n], pool=cache.pool, table=cache.table, seq_lens=[length], window=window, kind=kx.F32)
+    one = kx.paged_decode(cache.pool, cache.table, [length], got_q[-1:], window=window)
+    for h in range(2):
+        want, spread, size = exact_attention(got_q[:, h], ks[:, 0], vs[:, 0], seen, hs ** -0.5)
+        close(got[:, h], want, spread, size, 0, kx.F32)
+        close(one[:, h], want[-1:], spread[-1:], size[-1:], 2.0 ** -20, kx.F32)
+    one = kx.paged_decode(cache.pool, cache.table, [20 + window], got_q[-1:], window=window)
+    assert (one == 0).all()
 
 
 # ------------------------------------------------------------------ one new token per sequence
@@ -673,3 +705,111 @@ def test_calls_on_two_streams():
     for cache, q, x, b, *_ in jobs:
         check_decode(cache, q, b["out"].numpy(), 0, 0.125, kx.F32)
         check_logprobs(x, None, 4, (None, b["e"].numpy(), b["ids"].numpy(), b["tl"].numpy()), kx.F32)
+
+
+@pytest.mark.parametrize("kind", [kx.F32, kx.F16], ids=lambda k: NAMES[k])
+def test_windows_longer_than_anything(kind):
+    """A window of 2^31 - 1 is none, with rows ahead of the first key as well."""
+    rng = np.random.default_rng(81)
+    cu, ck = [0, 90, 160], [0, 20, 220]
+    q, k, v = (rounded(rng.standard_normal((n, m, 64)).astype(np.float32), kind) for n, m in ((160, 4), (220, 2), (220, 2)))
+    parts = [(k[a:b], v[a:b]) for a, b in ((0, 20), (20, 220))]
+    got = kx.prompt_attention(q, cu, k, v, cu_k=ck, window=2 ** 31 - 1, kind=kind)
+    check_prompt(q, cu, [p[0] for p in parts], [p[1] for p in parts], got, kind, 0.125)
+    assert (got[:70] == 0).all() and (got[70:90] != 0).all()
+    cache = Cache(rng, [1, 300], 2, 64, 16, kind)
+    got = kx.paged_decode(cache.pool, cache.table, cache.lens, q[:2], window=2 ** 31 - 1, q_kind=kind)
+    check_decode(cache, q[:2], got, 0, 0.125, kind)
+
+
+def test_one_workspace_for_all_that_meet_in_it():
+    """Decode and log probabilities of several sizes take turns in one workspace."""
+    rng = np.random.default_rng(82)
+    L = kx.lib()
+    ws = kx.Buf.zeros(max(L.kx_paged_decode_workspace_bytes(9, 40, 8, 128), L.kx_paged_decode_workspace_bytes(1, 4, 1, 64),
+                          L.kx_token_logprobs_workspace_bytes(512, 5000, 32)), np.uint8)
+    wide, one = Cache(rng, [900, 40, 7000] + [5] * 6, 8, 128, 16, kx.BF16), Cache(rng, [9000], 1, 64, 16, kx.F16)
+    q, q1 = rng.standard_normal((9, 40, 128)).astype(np.float32), rng.standard_normal((1, 4, 64)).astype(np.float32)
+    few, many = (rng.standard_normal((2, 90000)) * 3).astype(np.float32), rng.standard_normal((512, 5000)).astype(np.float32)
+    first = None
+    for turn in range(3):
+        got = (kx.paged_decode(wide.pool, wide.table, wide.lens, q, workspace=ws),
+               *kx.token_logprobs(many, None, 32, workspace=ws)[1:],
+               kx.paged_decode(one.pool, one.table, one.lens, q1, workspace=ws),
+               *kx.token_logprobs(few, None, 5, workspace=ws)[1:])
+        if turn == 0:
+            first = got
+            check_decode(wide, q, got[0], 0, 128 ** -0.5, kx.F32)
+            check_decode(one, q1, got[4], 0, 0.125, kx.F32)
+            check_logprobs(many, None, 32, (None, *got[1:4]), kx.F32)
+            check_logprobs(few, None, 5, (None, *got[5:]), kx.F32)
+        for a, b in zip(first, got):
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("kind", [kx.F32, kx.F16, kx.BF16], ids=lambda k: NAMES[k])
+def test_a_step_captured_and_replayed(kind):
+    """Filing, attention of the new rows, attention of the last one and the log probabilities as one graph, replayed as
+    the rows' dealing over the sequences, the lengths and the pages change; each replay against eager calls."""
+    rng = np.random.default_rng(83)
+    heads, kv_heads, hs, page, rows, batch, vocab = 8, 2, 64, 16, 48, 3, 40000
+    width, wide = KINDW[kind], kx.KIND_DTYPE[kind]
+    pages = np.zeros((60, page, kv_heads, hs), np.float32)
+    pool, other = kx.PagePool(pages, pages, kind), kx.PagePool(pages, pages, kind)
+    tables = rope_tables(400, hs)
+    sin, cos = (kx.Buf.from_numpy(t) for t in tables)
+    b = dict(k=kx.Buf(rows * kv_heads * hs * width), v=kx.Buf(rows * kv_heads * hs * width), q=kx.Buf(rows * heads * hs * width),
+             qo=kx.Buf.zeros((rows, heads, hs), wide), o=kx.Buf.zeros((rows, heads, hs), wide), d=kx.Buf.zeros((batch, heads, hs), wide),
+             x=kx.Buf(batch * vocab * width), lp=kx.Buf.zeros(batch), en=kx.Buf.zeros(batch), ids=kx.Buf.zeros((batch, 4), np.int32),
+             tl=kx.Buf.zeros((batch, 4)))
+    table, lens, cu = kx.Buf.zeros((batch, 20), np.int32), kx.Buf.zeros(batch, np.int32), kx.Buf.zeros(batch + 1, np.int32)
+    token = kx.Buf.zeros(batch, np.int32)
+    L = kx.lib()
+    ws = kx.Buf.zeros(max(L.kx_paged_decode_workspace_bytes(batch, heads, kv_heads, hs), L.kx_token_logprobs_workspace_bytes(batch, vocab, 4)), np.uint8)
+    kv = pool.desc(table, lens)
+    n, m = heads * hs, kv_heads * hs
+    w = kx.PagedWriteDesc(kv=kv, src_type=kind, rows=rows, head_num=heads, rope_variant=1, table_rows=400, cu_rows=cu.ptr,
+                          k=b["k"].ptr, k_stride=m, v=b["v"].ptr, v_stride=m, q=b["q"].ptr, q_stride=n, q_out=b["qo"].ptr,
+                          q_out_stride=n, sin_cache=sin.ptr, cos_cache=cos.ptr)
+    p = kx.PromptAttnDesc(type=kind, head_num=heads, kv_head_num=kv_heads, head_size=hs, batch=batch, q_rows=rows, causal=1,
+                          scale=0.125, q=b["qo"].ptr, q_stride=n, out=b["o"].ptr, out_stride=n, cu_q=cu.ptr, pages=C.addressof(kv))
+    d = kx.PagedDecodeDesc(kv=kv, q_type=kind, head_num=heads, scale=0.125, q=b["qo"].ptr, q_stride=n, out=b["d"].ptr,
+                           out_stride=n, workspace=ws.ptr, workspace_bytes=ws.nbytes)
+    x = kx.LogprobsDesc(type=kind, rows=batch, vocab=vocab, top_n=4, logits=b["x"].ptr, row_stride=vocab, tokens=token.ptr,
+                        logprob=b["lp"].ptr, entropy=b["en"].ptr, top_ids=b["ids"].ptr, top_logprobs=b["tl"].ptr,
+                        workspace=ws.ptr, workspace_bytes=ws.nbytes)
+    stream, graph = kx.Stream(), C.c_void_p()
+    kx.check(L.kx_graph_begin_capture(stream.ptr))
+    for f, what in ((L.kx_paged_write, w), (L.kx_prompt_attention, p), (L.kx_paged_decode, d), (L.kx_token_logprobs, x)):
+        kx.check(f(C.byref(what), stream.ptr))
+    kx.check(L.kx_graph_end_capture(stream.ptr, C.byref(graph)))
+    have = np.zeros(batch, int)
+    where = rng.permutation(60).reshape(batch, 20).astype(np.int32)
+    table.upload(where)
+    for new in ([16, 16, 16], [48, 0, 0], [1, 1, 1], [0, 40, 8], [3, 20, 25], [1, 0, 2]):
+        have += new
+        bounds = np.cumsum([0] + new)
+        q, k, v = (rounded(rng.standard_normal((rows, g, hs)).astype(np.float32), kind) for g in (heads, kv_heads, kv_heads))
+        logits, tokens = rounded((rng.standard_normal((batch, vocab)) * 3).astype(np.float32), kind), rng.integers(0, vocab, batch)
+        for name, a in (("q", q), ("k", k), ("v", v), ("x", logits)):
+            b[name].upload(kx.to_kind(a, kind))
+        cu.upload(bounds.astype(np.int32))
+        lens.upload(have.astype(np.int32))
+        token.upload(tokens.astype(np.int32))
+        kx.check(L.kx_graph_launch(graph, stream.ptr))
+        stream.sync()
+        last = bounds[-1]
+        eager_q = kx.paged_write(other, where, have, bounds, k, v, q, tables, 1, kind)
+        for a, c in zip(pool.read(), other.read()):
+            np.testing.assert_array_equal(a, c)
+        got_q, out = (kx.from_kind(b[name].numpy(wide, (rows, heads, hs)), kind) for name in ("qo", "o"))
+        np.testing.assert_array_equal(got_q[:last], eager_q[:last])
+        eager = kx.prompt_attention(eager_q, bounds, pool=other, table=where, seq_lens=have, scale=0.125, kind=kind)
+        np.testing.assert_array_equal(out[:last], eager[:last])
+        one = kx.paged_decode(other, where, have, got_q[:batch], scale=0.125, q_kind=kind)
+        np.testing.assert_array_equal(kx.from_kind(b["d"].numpy(wide, (batch, heads, hs)), kind), one)
+        said = kx.token_logprobs(logits, tokens, 4, kind)
+        for a, c in zip(said, (b["lp"].numpy(), b["en"].numpy(), b["ids"].numpy(), b["tl"].numpy())):
+            np.testing.assert_array_equal(a, c)
+        check_logprobs(logits, tokens, 4, said, kind)
+    L.kx_graph_destroy(graph)

@@ -5,7 +5,7 @@ import pytest
 
 import kx
 
-EINVAL, EUNSUPPORTED, EWORKSPACE = -1, -2, -3
+EINVAL, EUNSUPPORTED, EWORKSPACE, ELIMIT = -1, -2, -3, -4
 P = 1 << 20  # a 16-byte aligned address that nothing reads
 
 
@@ -22,7 +22,8 @@ BAD_PAGES = [(dict(type=3), EINVAL), (dict(type=-1), EINVAL), (dict(kv_head_num=
              (dict(table=P + 1), EINVAL), (dict(seq_lens=None), EINVAL), (dict(head_size=48), EUNSUPPORTED),
              (dict(head_size=0), EUNSUPPORTED), (dict(page_stride=32), EINVAL), (dict(row_stride=132), EINVAL),
              (dict(head_stride=0), EINVAL), (dict(table_stride=3), EINVAL), (dict(batch=-1), EINVAL),
-             (dict(page_size=1 << 16, table_pages=1 << 15, table_stride=1 << 15), EINVAL)]
+             (dict(page_size=1 << 16, table_pages=1 << 15, table_stride=1 << 15), EINVAL),
+             (dict(page_size=0x7FFFFF01, table_pages=1), EINVAL)]
 
 
 def write(kv=None, **kw):
@@ -68,7 +69,8 @@ def test_pages(bad, code):
     (dict(k_stride=130), EINVAL), (dict(v_stride=0), EINVAL), (dict(q_out=None), EINVAL), (dict(q=None), EINVAL),
     (dict(q_stride=252), EINVAL), (dict(q_out_stride=258), EINVAL), (dict(q=P + 8), EINVAL), (dict(q_out=P + 8), EINVAL), (dict(head_num=0), EINVAL),
     (dict(sin_cache=None), EINVAL), (dict(cos_cache=None), EINVAL), (dict(sin_cache=None, cos_cache=None), EINVAL),
-    (dict(table_rows=0), EINVAL), (dict(rope_variant=2), EINVAL)])
+    (dict(table_rows=0), EINVAL), (dict(rope_variant=2), EINVAL), (dict(q_out_stride=264), EINVAL), (dict(rows=1 << 25), ELIMIT),
+    (dict(head_num=1 << 24, q_stride=1 << 30, q_out_stride=1 << 30), ELIMIT)])
 def test_write(bad, code):
     assert write(**bad) == code
 
@@ -77,7 +79,7 @@ def test_write(bad, code):
     (dict(q_type=5), EINVAL), (dict(q_type=kx.BF16), EUNSUPPORTED), (dict(head_num=3), EINVAL), (dict(head_num=0), EINVAL),
     (dict(window=-1), EINVAL), (dict(q=None), EINVAL), (dict(out=None), EINVAL), (dict(q=P + 4), EINVAL),
     (dict(out=P + 8), EINVAL), (dict(q_stride=255), EINVAL), (dict(q_stride=258), EINVAL), (dict(out_stride=128), EINVAL),
-    (dict(workspace=None), EWORKSPACE), (dict(workspace=P + 16), EINVAL), (dict(workspace_bytes=64), EWORKSPACE)])
+    (dict(workspace=None), EWORKSPACE), (dict(workspace=P + 16), EINVAL), (dict(workspace_bytes=64), EWORKSPACE), (dict(scale=float("nan")), EINVAL), (dict(scale=float("inf")), EINVAL)])
 def test_decode(bad, code):
     assert decode(**bad) == code
 
@@ -88,9 +90,22 @@ def test_decode(bad, code):
     (dict(window=4, causal=0), EINVAL), (dict(q=None), EINVAL), (dict(k=None), EINVAL), (dict(v=None), EINVAL),
     (dict(out=None), EINVAL), (dict(cu_q=None), EINVAL), (dict(cu_k=None), EINVAL), (dict(cu_q=P + 2), EINVAL),
     (dict(q=P + 2), EINVAL), (dict(v=P + 8), EINVAL), (dict(q_stride=260), EINVAL), (dict(k_stride=120), EINVAL),
-    (dict(v_stride=132), EINVAL), (dict(out_stride=0), EINVAL)])
+    (dict(v_stride=132), EINVAL), (dict(out_stride=0), EINVAL), (dict(scale=float("nan")), EINVAL),
+    (dict(k_stride=1 << 22), EUNSUPPORTED), (dict(v_stride=1 << 22), EUNSUPPORTED), (dict(q_rows=1 << 30), ELIMIT),
+    (dict(k_rows=0x7FFFFF01), ELIMIT), (dict(q_rows=1 << 30, head_num=2), ELIMIT), (dict(batch=1 << 22), ELIMIT)])
 def test_prompt(bad, code):
     assert prompt(**bad) == code
+
+
+@pytest.mark.parametrize("bad", [dict(page_stride=1 << 31), dict(row_stride=1 << 26)])
+def test_prompt_over_pages_far_apart(bad):
+    p = pages(**bad)
+    assert prompt(k=None, v=None, cu_k=None, pages=C.addressof(p)) == EUNSUPPORTED
+
+
+@pytest.mark.parametrize("heads,batch,code", [(1025, 2, EUNSUPPORTED), (2, 1 << 23, ELIMIT)])
+def test_decode_limits(heads, batch, code):
+    assert decode(kv=pages(kv_head_num=heads, batch=batch), head_num=heads, q_stride=heads * 64, out_stride=heads * 64) == code
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -107,7 +122,8 @@ def test_prompt_over_pages(bad, code):
     (dict(logits=None), EINVAL), (dict(logits=P + 2), EINVAL), (dict(tokens=None), EINVAL), (dict(logprob=None), EINVAL),
     (dict(top_n=-1), EINVAL), (dict(top_n=33), EINVAL), (dict(top_n=6, vocab=5), EINVAL), (dict(top_ids=None), EINVAL),
     (dict(top_logprobs=None), EINVAL), (dict(workspace=None), EWORKSPACE), (dict(workspace=P + 8), EINVAL),
-    (dict(workspace_bytes=16), EWORKSPACE)])
+    (dict(workspace_bytes=16), EWORKSPACE), (dict(rows=1 << 24), ELIMIT),
+    (dict(vocab=0x7FFFFF01, row_stride=0x7FFFFF01), ELIMIT)])
 def test_logprobs(bad, code):
     assert logprobs(**bad) == code
 
