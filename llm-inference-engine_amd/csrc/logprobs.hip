@@ -3,15 +3,16 @@
 //   m = a reference near max x,  z = sum e^{x - m},  s = sum (x - m) e^{x - m}
 //   log p_t = (x_t - m) - ln z,   entropy = ln z - s / z
 //
-// Bound: the row is read once (rows * vocab * element size); about ten vector instructions per element, four of them the
-// exponential, are three quarters of that time for 16-bit logits.
+// Bound: the row is read once (rows * vocab * element size): 623 MB of 16-bit logits in 118 us, 5.3 TB/s, where a plain sum
+// over as much memory reads 5.7.  About nine vector instructions per element take two thirds of that time.
 //
 // Split: a workgroup takes a row, or with few rows one of up to 32 parts of it; the parts' sums and lists meet in the
 // workspace and the workgroup that arrives last joins them in their order.
 //
 // Alternatives without a second pass: a lane keeps its largest value of all and of each of eight groups of its loads.  The
 // top_n-th largest of a wave's 64 lane maxima is at most the top_n-th largest value, so only the few groups that
-// reach it are read again (they are in the caches), and their elements at or above it (some tens) are ranked by counting.
+// reach it are read again (they are in the caches), their elements dealt over all threads (a wave that walked its lanes'
+// groups by itself did so for 64 lanes each time: 142 us instead of 118), and those at or above it (some tens) are ranked by counting.
 // Where more of them are alike than the list holds, the part is gone through in order of index instead.
 //
 // The reference m is shared by a wave and follows a new maximum only when that lies more than 16 above it (e^16 is far
@@ -134,7 +135,8 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
   unsigned long long* sm_list = sm_raw + kLpGroups * kLpThreads / 2;
   __shared__ unsigned long long sm_top[KX_LOGPROBS_TOP_MAX];
   __shared__ float sm_sums[kLpWaves][3], sm_least[kLpWaves];
-  __shared__ int sm_count, sm_last;
+  __shared__ unsigned short sm_hit[kLpList];  // groups to look through: group * threads + thread
+  __shared__ int sm_count, sm_hits, sm_last;
 
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
   if (part == a.parts - 1 && tid >= 8 && behind0 + tid - 8 < a.vocab) extra = behind0 + tid - 8;
   const float xe = extra >= 0 ? (float)*KX_CK(a, PL_X, x + extra) : -INFINITY;
 
-  if (tid == 0) sm_count = 0;
+  if (tid == 0) sm_count = sm_hits = 0;
   LogSums sums = {wave_max(xe), 0.f, 0.f};
   float largest = fmaxf(xe, -INFINITY);  // (no NaN)
   if (extra >= 0) {
@@ -239,34 +241,49 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
       const int at = atomicAdd(&sm_count, 1);
       if (at < kLpList) sm_list[at] = key_of(xe, extra);
     }
-    for (int group = 0; group * group_steps < steps; ++group) {
-      if (sm_group[group * kLpThreads + tid] < least) continue;
-      for (int st = group * group_steps; st < min((group + 1) * group_steps, steps); ++st) {
-        // fp32: the whole step, which is still at hand if it is the only one; 16-bit types: a vector at a time (registers
-        // are dearer than the wait)
-        constexpr int AT_ONCE = N == 4 ? kLpUnroll : 1;
-#pragma unroll 1
-        for (int u0 = 0; u0 < kLpUnroll; u0 += AT_ONCE) {
-          const int first = v0 + st * per_step + u0 * kLpThreads + tid;
-          if (N == 8) v[0] = *KX_CK(a, PL_X, xv + min(first, v1 - 1));
-          else if (steps > 1) load_step(st, v);
-          unsigned hits = 0;
+    if (N == 4 && steps == 1) {  // the elements are still at hand
+      unsigned hits = 0;
 #pragma unroll
-          for (int u = 0; u < AT_ONCE; ++u)
+      for (int u = 0; u < kLpUnroll; ++u)
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (!(Vec::get(v[u], e) < least) && first + u * kLpThreads < v1) hits |= 1u << (u * N + e);
-          if (!hits) continue;
-          int at = atomicAdd(&sm_count, __builtin_popcount(hits));
+        for (int e = 0; e < N; ++e)
+          if (!(Vec::get(v[u], e) < least) && v0 + tid + u * kLpThreads < v1) hits |= 1u << (u * N + e);
+      if (hits) {
+        int at = atomicAdd(&sm_count, __builtin_popcount(hits));
 #pragma unroll
-          for (int u = 0; u < AT_ONCE; ++u)
+        for (int u = 0; u < kLpUnroll; ++u)
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (hits >> (u * N + e) & 1) {
-                if (at < kLpList) sm_list[at] = key_of(Vec::get(v[u], e), ahead + (first + u * kLpThreads) * N + e);
-                ++at;
-              }
+          for (int e = 0; e < N; ++e)
+            if (hits >> (u * N + e) & 1) {
+              if (at < kLpList) sm_list[at] = key_of(Vec::get(v[u], e), ahead + (v0 + tid + u * kLpThreads) * N + e);
+              ++at;
+            }
+      }
+    } else {
+      // the groups that reach it, and then all of their elements, dealt over the threads
+      for (int group = 0; group * group_steps < steps; ++group)
+        if (!(sm_group[group * kLpThreads + tid] < least)) {
+          const int at = atomicAdd(&sm_hits, 1);
+          if (at < kLpList) sm_hit[at] = (unsigned short)(group * kLpThreads + tid);
         }
+      __syncthreads();
+      if (sm_hits <= kLpList) {
+        constexpr int PER = kLpUnroll * N;  // elements of a step
+        for (int i = tid; i < sm_hits * PER; i += kLpThreads) {
+          const int hit = sm_hit[i / PER], e = i % PER, group = hit / kLpThreads;
+          const int end = min((group + 1) * group_steps, steps);
+          for (int st = group * group_steps; st < end; ++st) {
+            const int vec = v0 + st * per_step + e / N * kLpThreads + hit % kLpThreads;
+            if (vec >= v1) continue;
+            const int index = ahead + vec * N + e % N;
+            const float value = (float)*KX_CK(a, PL_X, x + index);
+            if (value < least) continue;
+            const int at = atomicAdd(&sm_count, 1);
+            if (at < kLpList) sm_list[at] = key_of(value, index);
+          }
+        }
+      } else if (tid == 0) {
+        sm_count = kLpList + 1;  // each of them holds an element of the list at least
       }
     }
     __syncthreads();
