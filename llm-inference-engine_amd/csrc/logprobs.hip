@@ -3,16 +3,18 @@
 //   m = a reference near max x,  z = sum e^{x - m},  s = sum (x - m) e^{x - m}
 //   log p_t = (x_t - m) - ln z,   entropy = ln z - s / z
 //
-// Bound: the row is read once (rows * vocab * element size): 623 MB of 16-bit logits in 118 us, 5.3 TB/s, where a plain sum
-// over as much memory reads 5.7.  About nine vector instructions per element take two thirds of that time.
+// Bound: the row is read once (rows * vocab * element size): 623 MB of 16-bit logits in 116 us, 5.4 TB/s, where a plain sum
+// over as much memory reads 5.7.  About eight vector instructions per element take two thirds of that time.  A single row
+// of 128 k fp32 logits takes 7.9 us, latencies of loads, of the ticket and of code that runs once.
 //
 // Split: a workgroup takes a row, or with few rows one of up to 32 parts of it; the parts' sums and lists meet in the
 // workspace and the workgroup that arrives last joins them in their order.
 //
 // Alternatives without a second pass: a lane keeps its largest value of all and of each of eight groups of its loads.  The
-// top_n-th largest of a wave's 64 lane maxima is at most the top_n-th largest value, so only the few groups that
-// reach it are read again (they are in the caches), their elements dealt over all threads (a wave that walked its lanes'
-// groups by itself did so for 64 lanes each time: 142 us instead of 118), and those at or above it (some tens) are ranked by counting.
+// top_n-th largest of 64 of them (the largest of four lanes each) is at most the top_n-th largest value, so only the few
+// groups that reach it are read again (they are in the caches), their elements dealt over all threads (a wave that walked
+// its lanes' groups by itself did so for 64 lanes each time: 142 us instead of 118; elements kept in registers instead, each
+// with its own code: 11.2 us for the single row), and those at or above it (some tens) are ranked by counting.
 // Where more of them are alike than the list holds, the part is gone through in order of index instead.
 //
 // The reference m is shared by a wave and follows a new maximum only when that lies more than 16 above it (e^16 is far
@@ -56,11 +58,11 @@ __device__ __forceinline__ unsigned order_of(float x) {
 }
 __device__ __forceinline__ float value_of_order(unsigned u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
 
-// At most the n-th largest of the wave's values: its first 20 bits, found from the top (0 with fewer than n above it).
+// At most the n-th largest of the wave's values: its first 16 bits, found from the top (0 with fewer than n above it).
 __device__ __forceinline__ unsigned nth_largest(unsigned v, int n) {
   unsigned t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 12; --bit) {
+  for (int bit = 31; bit >= 16; --bit) {
     const unsigned c = t | 1u << bit;
     if (__builtin_popcountll(__ballot(v >= c)) >= n) t = c;
   }
@@ -111,14 +113,18 @@ __device__ __forceinline__ void rebase(LogSums& a, float m) {
   a.m = m;
 }
 
-// The top_n largest of the `count` keys in LDS, in falling order: a key's place is the number of keys above it.
+// The top_n largest of the `count` keys in LDS, in falling order: a key's place is the number of keys above it, which four
+// lanes count together.
 __device__ __forceinline__ void rank_keys(const unsigned long long* keys, int count, int top_n, unsigned long long* out) {
-  for (int i = threadIdx.x; i < count; i += kLpThreads) {
+  const int part = threadIdx.x % 4;
+  for (int i = threadIdx.x / 4; i < count; i += kLpThreads / 4) {
     const unsigned long long mine = keys[i];
     int above = 0;
-#pragma unroll 8
-    for (int j = 0; j < count; ++j) above += keys[j] > mine;
-    if (above < top_n) out[above] = mine;
+#pragma unroll 4
+    for (int j = part; j < count; j += 4) above += keys[j] > mine;
+    above += __builtin_amdgcn_update_dpp(0, above, 0xB1, 0xF, 0xF, true);  // the lane's neighbour of a pair
+    above += __builtin_amdgcn_update_dpp(0, above, 0x4E, 0xF, 0xF, true);  // the other pair of four
+    if (part == 0 && above < top_n) out[above] = mine;
   }
 }
 
@@ -134,7 +140,8 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
   float* sm_group = reinterpret_cast<float*>(sm_raw);
   unsigned long long* sm_list = sm_raw + kLpGroups * kLpThreads / 2;
   __shared__ unsigned long long sm_top[KX_LOGPROBS_TOP_MAX];
-  __shared__ float sm_sums[kLpWaves][3], sm_least[kLpWaves];
+  __shared__ float sm_sums[kLpWaves][3];
+  __shared__ unsigned sm_largest[kLpThreads];
   __shared__ unsigned short sm_hit[kLpList];  // groups to look through: group * threads + thread
   __shared__ int sm_count, sm_hits, sm_last;
 
@@ -175,11 +182,11 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     }
   };
   int step = 0;
-  u32x4 v[kLpUnroll];  // (fp32: the elements of an only step stay for the search below)
   for (int group = 0; step < steps; ++group) {
     float group_max = -INFINITY;
     const int end = min(step + group_steps, steps);
     for (; step < end; ++step) {
+      u32x4 v[kLpUnroll];
       load_step(step, v);
       float mx = Vec::get(v[0], 0);
 #pragma unroll
@@ -215,11 +222,7 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     sm_sums[wave][1] = sums.z;
     sm_sums[wave][2] = sums.s;
   }
-  if (a.top_n > 0) {
-    // (a bound below every value is a NaN here, which no value is below)
-    const float bound = value_of_order(nth_largest(order_of(largest), a.top_n));
-    if (lane == 0) sm_least[wave] = bound;
-  }
+  if (a.top_n > 0) sm_largest[tid] = order_of(largest);
   __syncthreads();
   LogSums all = {-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -233,58 +236,49 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
   }
 
   if (a.top_n > 0) {
-    float least = sm_least[0];
+    unsigned of_lanes = sm_largest[lane];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w) least = fmaxf(least, sm_least[w]);
+    for (int w = 1; w < kLpWaves; ++w) of_lanes = max(of_lanes, sm_largest[w * 64 + lane]);
+    // (a bound below every value is a NaN here, which no value is below)
+    const float least = value_of_order(nth_largest(of_lanes, a.top_n));
     // not below it (a NaN may be among the best of a row with fewer than top_n others)
     if (extra >= 0 && !(xe < least)) {
       const int at = atomicAdd(&sm_count, 1);
       if (at < kLpList) sm_list[at] = key_of(xe, extra);
     }
-    if (N == 4 && steps == 1) {  // the elements are still at hand
-      unsigned hits = 0;
-#pragma unroll
-      for (int u = 0; u < kLpUnroll; ++u)
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (!(Vec::get(v[u], e) < least) && v0 + tid + u * kLpThreads < v1) hits |= 1u << (u * N + e);
-      if (hits) {
-        int at = atomicAdd(&sm_count, __builtin_popcount(hits));
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u)
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (hits >> (u * N + e) & 1) {
-              if (at < kLpList) sm_list[at] = key_of(Vec::get(v[u], e), ahead + (v0 + tid + u * kLpThreads) * N + e);
-              ++at;
-            }
+    // the groups that reach it, and then all of their elements, dealt over the threads
+    for (int group = 0; group * group_steps < steps; ++group)
+      if (!(sm_group[group * kLpThreads + tid] < least)) {
+        const int at = atomicAdd(&sm_hits, 1);
+        if (at < kLpList) sm_hit[at] = (unsigned short)(group * kLpThreads + tid);
       }
-    } else {
-      // the groups that reach it, and then all of their elements, dealt over the threads
-      for (int group = 0; group * group_steps < steps; ++group)
-        if (!(sm_group[group * kLpThreads + tid] < least)) {
-          const int at = atomicAdd(&sm_hits, 1);
-          if (at < kLpList) sm_hit[at] = (unsigned short)(group * kLpThreads + tid);
-        }
-      __syncthreads();
-      if (sm_hits <= kLpList) {
-        constexpr int PER = kLpUnroll * N;  // elements of a step
-        for (int i = tid; i < sm_hits * PER; i += kLpThreads) {
-          const int hit = sm_hit[i / PER], e = i % PER, group = hit / kLpThreads;
-          const int end = min((group + 1) * group_steps, steps);
-          for (int st = group * group_steps; st < end; ++st) {
-            const int vec = v0 + st * per_step + e / N * kLpThreads + hit % kLpThreads;
-            if (vec >= v1) continue;
-            const int index = ahead + vec * N + e % N;
-            const float value = (float)*KX_CK(a, PL_X, x + index);
-            if (value < least) continue;
-            const int at = atomicAdd(&sm_count, 1);
-            if (at < kLpList) sm_list[at] = key_of(value, index);
+    __syncthreads();
+    if (sm_hits <= kLpList) {
+      constexpr int PER = kLpUnroll * N;  // elements of a step
+      constexpr int AT_ONCE = 2;
+      const int elements = sm_hits * PER;
+      for (int i0 = tid; i0 < elements; i0 += AT_ONCE * kLpThreads) {
+        for (int st = 0; st < group_steps; ++st) {
+          int index[AT_ONCE];
+          float value[AT_ONCE];
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            const int i = min(i0 + k * kLpThreads, elements - 1), hit = sm_hit[i / PER], e = i % PER;
+            const int step_of = hit / kLpThreads * group_steps + st, vec = v0 + step_of * per_step + e / N * kLpThreads + hit % kLpThreads;
+            const bool mine = i0 + k * kLpThreads < elements && vec < v1;
+            index[k] = mine ? ahead + vec * N + e % N : -1;
+            value[k] = (float)*KX_CK(a, PL_X, x + max(index[k], 0));
           }
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k)
+            if (index[k] >= 0 && !(value[k] < least)) {
+              const int at = atomicAdd(&sm_count, 1);
+              if (at < kLpList) sm_list[at] = key_of(value[k], index[k]);
+            }
         }
-      } else if (tid == 0) {
-        sm_count = kLpList + 1;  // each of them holds an element of the list at least
       }
+    } else if (tid == 0) {
+      sm_count = kLpList + 1;  // each of them holds an element of the list at least
     }
     __syncthreads();
     int count = sm_count;
