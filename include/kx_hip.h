@@ -651,7 +651,8 @@ int kx_paged_write(const kx_paged_write_desc* desc, void* stream);
 /* Attention of one new token per sequence over its pages (kx_mha_decode_f32 for a batch): for head h of
  * sequence b, over the positions max(0, seq_lens[b] - window) <= t < seq_lens[b] (window 0: all),
  *   out[b][h] = sum_t softmax_t(scale * q[b][h] . K_b[t][h / (head_num / kv_head_num)]) * V_b[t][..]
- * in fp32 arithmetic; zeros where no position is seen.  q and out rows of head_num * head_size at their
+ * in fp32 arithmetic; zeros where no position is seen.  (An infinity among the seen keys and values may give NaN
+ * where the formula has a limit; what is not seen may hold anything.)  q and out rows of head_num * head_size at their
  * strides (elements, multiples of 16 bytes), of type q_type: KX_F32 over any cache, KX_F16 / KX_BF16 over
  * a cache of the same type.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
  * must be ZERO before its first use and is left ready for the next call by every call; calls that

@@ -17,10 +17,12 @@
 // value per lane and the weights are already the B operand of O^T = V^T P^T; the A operand V^T comes out of row-major V by
 // transposing LDS reads (16-bit types), or one element per lane (fp32).
 //
-// Reached: 1.0 PFLOP/s on a prompt of 4096 (32 heads over 8, 128 wide, bf16: 134 us), at 2.0 GHz: the chip's power, which holds
+// Reached: 1.0 PFLOP/s on a prompt of 4096 (32 heads over 8, 128 wide, bf16: 135 us), at 2.0 GHz: the chip's power, which holds
 // a library product of 8192 x 8192 x 8192 to 1.09 PFLOP/s as well.  Half the cycles are matrix instructions and half vector
 // ones there.  Tried and no faster: the two waves of a SIMD half a step apart (150 us), the next scores and the last
-// second product between a wave's vector instructions (143, with spills), waiting later for the LDS-DMA (the same).
+// second product between a wave's vector instructions (143, with spills), waiting later for the LDS-DMA (the same), two
+// workgroups of four waves and 32-key tiles per CU (154), the sum of the weights by dot products (133; 93 for the pieces, 91 now).
+// A workgroup takes 7 us beside its tiles (lengths, pages and first tiles 4, joining and storing 2).
 //
 // Rounding: products of 16-bit operands are exact in fp32 and summed there, softmax in fp32, weights rounded to the
 // type for the second product, the sum of the weights unrounded.  The running maximum follows only when it is
@@ -86,7 +88,8 @@ __device__ __forceinline__ bool find_prompt(const PromptArgs& a, int item, Promp
       }
     }
     // The sequences (64 at a time) in falling order of their keys, each one's last blocks first: long chains of tiles
-    // start early.  (Six pieces of 118 .. 1024 rows over 425 .. 4298 keys: 178 us in index order, 146 so, one group.)
+    // start early.  (Six pieces of 118 .. 1024 rows over 425 .. 4298 keys: 178 us in index order, 146 so, in the form that this was
+    // tried with, now 91.)
     const int mine = (int)(((int64_t)n * a.kv_mul + ROWS - 1) / ROWS);
     int blocks = mine, from = lane;
     if (a.batch > 1) {
@@ -624,10 +627,10 @@ static int prompt_mode(const PromptArgs& a, hipStream_t s) {
 // Groups of waves per workgroup.  Two or more cut a sequence's chain of tiles and give that many times the workgroups, for
 // as many times the K/V traffic per product.
 //   16-bit: two groups where the call would not fill the chip with workgroups of 256 pairs (`blocks`) otherwise: under 320
-//   of them, or under 800 with 64-wide heads, whose smaller tiles let two such workgroups share a CU.  Measured (us,
-//   one group / two; causal, 32 heads over 8): 128 wide, blocks 64: 20.1 / 16.2, 256: 61.2 / 52.8, 375: 93 / 105, 512 (a
-//   prompt of 4096): 134 / 155; 64 wide, 128: 23.3 / 15.9, 473: 35.2 / 31.6, 1382: 103 / 116; 32 wide, 74: 35.2 / 21.1, 674:
-//   51.7 / 57.8.
+//   of them, or with narrower heads, whose smaller tiles let two such workgroups share a CU, under 800 (64 wide) or 600 (32).
+//   Measured (us, one group / two; causal, 32 heads over 8): 128 wide, blocks 64: 19.8 / 14.4, 256: 63.5 / 53.1, 346: 34.1 /
+//   37.9 (8 prompts), 375: 95.6 / 102, 512 (a prompt of 4096): 143 / 155; 64 wide, 85: 11.0 / 9.1, 473: 36.3 / 30.4, 512: 97.2 /
+//   87.7, 1090: 88.2 / 93.2, 2085: 134 / 151; 32 wide, 74: 34.4 / 20.2, 512: 76.9 / 63.0, 674: 51.7 / 57.8.
 //   fp32: as many groups as LDS holds buffers for, always: its products take sixteen times as long and hide the traffic
 //   (64 wide, blocks 31: one 33.7, two 26.8, four 18.9; 612: one 367, four 303; 128 wide, 512: one 1145, two 1097).
 template <typename T, int HS>
@@ -636,7 +639,7 @@ static int prompt_groups(const PromptArgs& a, hipStream_t s) {
     return prompt_mode<T, HS, prompt_lds<T, HS, 4>() <= 131072 ? 4 : 2>(a, s);
   } else {
     const double blocks = (double)a.q_rows * a.kv_mul / 256 * a.kv_heads;
-    return blocks < (HS == 64 ? 800 : 320) ? prompt_mode<T, HS, 2>(a, s) : prompt_mode<T, HS, 1>(a, s);
+    return blocks < (HS == 128 ? 320 : HS == 64 ? 800 : 600) ? prompt_mode<T, HS, 2>(a, s) : prompt_mode<T, HS, 1>(a, s);
   }
 }
 template <typename T>
