@@ -15,7 +15,8 @@
 // groups that reach it are read again (they are in the caches), their elements dealt over all threads (a wave that walked
 // its lanes' groups by itself did so for 64 lanes each time: 142 us instead of 118; elements kept in registers instead, each
 // with its own code: 11.2 us for the single row), and those at or above it (some tens) are ranked by counting.
-// Where more of them are alike than the list holds, the part is gone through in order of index instead.
+// Where more of them are alike than the list holds, or fewer than top_n are above -inf, the part is gone through in order of
+// index instead (the text with three logits a row that are not banned: 252 us).
 //
 // The reference m is shared by a wave and follows a new maximum only when that lies more than 16 above it (e^16 is far
 // from the range of fp32), so the sums are hardly ever rescaled.
@@ -285,26 +286,49 @@ __global__ __launch_bounds__(kLpThreads, 6) void logprobs_kernel(const LogprobsA
     if (tid < KX_LOGPROBS_TOP_MAX) sm_top[tid] = 0;
     __syncthreads();
     if (count > kLpList) {
-      // too many alike: in order of index, 256 at a time, the best so far kept at the head of the list
-      const int e0 = part == 0 ? 0 : ahead + v0 * N, e1 = part == a.parts - 1 ? a.vocab : ahead + v1 * N;
+      // Too many alike: in order of index, 256 at a time, the best so far kept at the head of the list.  A step without a
+      // value above the least of them (an equal one further on ranks below it) is passed over.
       unsigned long long least_key = 0;
       if (tid == 0) sm_count = 0;
       __syncthreads();
-      for (int base = e0; base < e1; base += kLpThreads) {
-        const int i = base + tid;
-        const unsigned long long key = i < e1 ? key_of((float)*KX_CK(a, PL_X, x + i), i) : 0;
-        if (key > least_key) sm_list[atomicAdd(&sm_count, 1)] = key;  // at most kLpList: see below
-        __syncthreads();
-        count = sm_count;
-        __syncthreads();
-        if (count > kLpList - kLpThreads) {
-          rank_keys(sm_list, count, a.top_n, sm_top);
+      auto look_through = [&](int from, int upto) {
+        for (int base = from; base < upto; base += kLpThreads) {
+          const int i = base + tid;
+          const unsigned long long key = i < upto ? key_of((float)*KX_CK(a, PL_X, x + i), i) : 0;
+          if (key > least_key) sm_list[atomicAdd(&sm_count, 1)] = key;  // at most kLpList: see below
           __syncthreads();
-          if (tid < a.top_n) sm_list[tid] = sm_top[tid];
-          least_key = sm_top[a.top_n - 1];
-          if (tid == 0) sm_count = a.top_n;
+          count = sm_count;
           __syncthreads();
+          if (count > kLpList - kLpThreads) {
+            rank_keys(sm_list, count, a.top_n, sm_top);
+            __syncthreads();
+            if (tid < a.top_n) sm_list[tid] = sm_top[tid];
+            least_key = sm_top[a.top_n - 1];
+            if (tid == 0) sm_count = a.top_n;
+            __syncthreads();
+          }
         }
+      };
+      // (the pieces one after the other: ahead of the vectors, a step of them each, behind them)
+      for (int st = -1; st <= steps; ++st) {
+        int from = part == 0 ? 0 : ahead, upto = ahead;
+        if (st == steps) {
+          from = behind0;
+          upto = part == a.parts - 1 ? a.vocab : behind0;
+        } else if (st >= 0) {
+          u32x4 v[kLpUnroll];
+          load_step(st, v);
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < kLpUnroll; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) mx = fmaxf(mx, Vec::get(v[u], e));
+          // (the value of no key is a NaN)
+          if (!__syncthreads_or(!(mx <= value_of_key(least_key)))) continue;
+          from = ahead + (v0 + st * per_step) * N;
+          upto = ahead + min(v0 + (st + 1) * per_step, v1) * N;
+        }
+        look_through(from, upto);
       }
       count = sm_count;
     }

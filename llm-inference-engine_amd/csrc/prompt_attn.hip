@@ -214,39 +214,10 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
     return (uint64_t)(page_ok(page) ? (unsigned)page : 0u) * page_bytes +
            (uint64_t)(unsigned)(t - a.kv.div.page(t) * a.kv.div.size) * row_bytes;
   };
-  // ---- queries: lane (pair, half) holds the pieces of its row that meet its pieces of a K row ----
-  typedef typename PromptMma<T>::frag frag;
-  frag qf[KS];
-  const T* qrow = reinterpret_cast<const T*>(a.q) + (w.q0 + my_row) * a.q_stride + (kvh * a.kv_mul + my_head) * HS;
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-    qf[ks] = *KX_CK(a, PP_Q, reinterpret_cast<const frag*>(reinterpret_cast<const char*>(qrow) + 32 * ks + 16 * half));
-  // A page that is not there is looked for once, beside the first tiles' way here, and tile by tile only if there is one.
-  const int last_col = PAGED && t0 < t1 ? a.kv.div.page(hi - 1) : 0, col = PAGED ? a.kv.div.page(lo) + (int)threadIdx.x : 0;
-  int probe = 0;
-  if (PAGED && t0 < t1) probe = *KX_CK(a, PP_TABLE, table + min(col, last_col));
-
   // The KG tiles of a buffer are consecutive, so its K rows are KG * KT consecutive keys.  DMA pair j of a wave, one
   // instruction for K and one for V: the first of its rows among the keys, and a lane's.
   auto pair_first = [&](int j) { return (wave + NW * j) * RPP; };
   auto pair_row = [&](int j) { return pair_first(j) + lane / CH; };
-  const bool has_pair = KP * KG >= NW || wave < KP * KG;
-  // a lane's byte offsets from the first row of the buffer (packed), from the first row of the instruction's 16-row block, or
-  // within its row (pages); `tail`: those in the last buffer, where rows behind the last key are replaced by it
-  unsigned k_off[RP], v_off[RP], k_tail[RP], v_tail[RP];
-  const int steps = (t1 - t0 + KG - 1) / KG, tail_key0 = (t0 + (steps - 1) * KG) * KT;
-#pragma unroll
-  for (int j = 0; j < RP; ++j) {
-    const int row = pair_row(j), from = MODE == PA_PACKED ? row : MODE == PA_BLOCK_PAGES ? lane / CH : 0;
-    const int block = min(tail_key0 + pair_first(j), (w.keys - 1) & ~(RPP - 1)) + lane / CH;
-    const int behind = MODE == PA_PACKED ? max(tail_key0 + row - (w.keys - 1), 0) : MODE == PA_BLOCK_PAGES ? max(block - (w.keys - 1), 0) : 0;
-    const unsigned kp = 16u * (lane % CH ^ k_swizzle<CH>(row)), vp = 16u * (lane % CH ^ v_swizzle<CH, F32>(row));
-    const unsigned kb = (unsigned)((int)k_stride * (int)sizeof(T)), vb = (unsigned)((int)v_stride * (int)sizeof(T));
-    k_off[j] = kp + from * kb;
-    v_off[j] = vp + from * vb;
-    k_tail[j] = kp + (unsigned)(from - behind) * kb;
-    v_tail[j] = vp + (unsigned)(from - behind) * vb;
-  }
   // Pages of the next buffer's rows, requested a step ahead: one per instruction where pages are whole 16-row blocks, else
   // one per lane.  (By vector loads in both cases: the end of a step waits for those anyway, while a scalar load would
   // have the next fragment reads wait for it.)
@@ -264,6 +235,36 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
       }
     }
   };
+  if (t0 < t1) get_ids(t0);
+  // ---- queries: lane (pair, half) holds the pieces of its row that meet its pieces of a K row ----
+  typedef typename PromptMma<T>::frag frag;
+  frag qf[KS];
+  const T* qrow = reinterpret_cast<const T*>(a.q) + (w.q0 + my_row) * a.q_stride + (kvh * a.kv_mul + my_head) * HS;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+    qf[ks] = *KX_CK(a, PP_Q, reinterpret_cast<const frag*>(reinterpret_cast<const char*>(qrow) + 32 * ks + 16 * half));
+  // A page that is not there is looked for once, beside the first tiles' way here, and tile by tile only if there is one.
+  const int last_col = PAGED && t0 < t1 ? a.kv.div.page(hi - 1) : 0, col = PAGED ? a.kv.div.page(lo) + (int)threadIdx.x : 0;
+  int probe = 0;
+  if (PAGED && t0 < t1) probe = *KX_CK(a, PP_TABLE, table + min(col, last_col));
+
+  const bool has_pair = KP * KG >= NW || wave < KP * KG;
+  // a lane's byte offsets from the first row of the buffer (packed), from the first row of the instruction's 16-row block, or
+  // within its row (pages); `tail`: those in the last buffer, where rows behind the last key are replaced by it
+  unsigned k_off[RP], v_off[RP], k_tail[RP], v_tail[RP];
+  const int steps = (t1 - t0 + KG - 1) / KG, tail_key0 = (t0 + (steps - 1) * KG) * KT;
+#pragma unroll
+  for (int j = 0; j < RP; ++j) {
+    const int row = pair_row(j), from = MODE == PA_PACKED ? row : MODE == PA_BLOCK_PAGES ? lane / CH : 0;
+    const int block = min(tail_key0 + pair_first(j), (w.keys - 1) & ~(RPP - 1)) + lane / CH;
+    const int behind = MODE == PA_PACKED ? max(tail_key0 + row - (w.keys - 1), 0) : MODE == PA_BLOCK_PAGES ? max(block - (w.keys - 1), 0) : 0;
+    const unsigned kp = 16u * (lane % CH ^ k_swizzle<CH>(row)), vp = 16u * (lane % CH ^ v_swizzle<CH, F32>(row));
+    const unsigned kb = (unsigned)((int)k_stride * (int)sizeof(T)), vb = (unsigned)((int)v_stride * (int)sizeof(T));
+    k_off[j] = kp + from * kb;
+    v_off[j] = vp + from * vb;
+    k_tail[j] = kp + (unsigned)(from - behind) * kb;
+    v_tail[j] = vp + (unsigned)(from - behind) * vb;
+  }
   auto issue = [&](int t, int buf, int from, int upto) {
     if (!has_pair) return;
     const int key0 = t * KT;
@@ -295,7 +296,6 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
   };
 
   if (t0 < t1) {
-    get_ids(t0);
     issue(t0, 0, 0, RP);
     if (t0 + KG < t1) get_ids(t0 + KG);
   }

@@ -591,6 +591,35 @@ def test_logprobs_orders(kind, rows):
 
 
 @pytest.mark.parametrize("kind", [kx.F32, kx.F16, kx.BF16], ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("rows,top_n", [(5, 32), (5, 5), (520, 5), (520, 32)])
+def test_logprobs_few_above_many_alike(kind, rows, top_n):
+    """A vocabulary of which next to nothing is allowed, or nearly all is alike, with the few at the ends, in the middle,
+    behind each other and in rising order; some rows hold NaN."""
+    vocab = 30011
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    at = np.array([0, 1, 255, 256, 4099, 8191, 8192, 20000, vocab - 9, vocab - 1])
+    for r in range(rows):
+        case = r % 5
+        if case in (1, 3, 4):
+            x[r] = 1.5
+        if case == 0:
+            x[r, at[[0, 5, 9]]] = 1.0
+        elif case == 1:
+            x[r, at] = 2.0 + np.arange(10)  # rising: each is above all ahead of it
+        elif case == 2:
+            x[r, vocab - 40:] = np.arange(40) * 0.25
+        elif case == 3:
+            x[r, at] = 1.5 - 0.5 * np.arange(10)
+            x[r, 777] = np.nan
+        else:
+            x[r, ::3] = -np.inf
+            x[r, at[::2]] = 3.0
+    tokens = np.where(np.arange(rows) % 2, vocab - 1, 8192)
+    got = kx.token_logprobs(x, tokens, top_n, kind, row_stride=vocab + 3)
+    check_logprobs(x, tokens, top_n, got, kind)
+
+
+@pytest.mark.parametrize("kind", [kx.F32, kx.F16, kx.BF16], ids=lambda k: NAMES[k])
 @pytest.mark.parametrize("rows", [8, 800])
 def test_logprobs_banned_and_broken_rows(kind, rows):
     vocab, rng = 4099, np.random.default_rng(18)
