@@ -625,7 +625,7 @@ typedef struct kx_paged_kv {
  * is outside 0 .. table_pages * page_size - 1, has no page or (when rotating) lies past table_rows is not filed; past
  * table_rows or below zero its q row is left alone too.  Rows of no sequence (below cu_rows[0], from cu_rows[batch] on) are left
  * alone.  No two rows of a call may have the same place in the pages.  Strides in elements, at least the
- * row's width and multiples of 16 bytes, q's and q_out's the same where they are one; pointers aligned to 16 bytes (KX_EINVAL).
+ * row's width and multiples of 16 bytes, q's and q_out's the same where they are one; pointers aligned to 16 bytes, the tables to 4 (KX_EINVAL).
  * KX_ELIMIT from 2^25 rows on, or for 2^30 elements of q, k and v in a row. */
 typedef struct kx_paged_write_desc {
   kx_paged_kv kv;
@@ -717,7 +717,7 @@ int kx_prompt_attention(const kx_prompt_attn_desc* desc, void* stream);
  *     among equal ones; NaN ranks below -inf         (top_n 0: NULL; top_n <= min(vocab, KX_LOGPROBS_TOP_MAX))
  * in fp32.  A token below zero is none: logprob 0; one past the vocabulary: NaN.  A row that is no
  * distribution (holds NaN or +inf, or nothing but -inf) gives NaN for the three kinds of numbers, and its ids in order.
- * Logits of `type`, rows at row_stride elements (any, >= vocab), aligned to their element.  workspace as for
+ * Logits of `type`, rows at row_stride elements (any, >= vocab), all arrays aligned to their elements.  workspace as for
  * kx_paged_decode, of kx_token_logprobs_workspace_bytes(rows, vocab, top_n) bytes.  KX_ELIMIT from 2^24 rows or 2^31 - 256
  * logits in a row on. */
 #define KX_LOGPROBS_TOP_MAX 32

@@ -436,6 +436,8 @@ extern "C" int kx_token_logprobs(const kx_logprobs_desc* d, void* stream) {
   if ((d->tokens != nullptr) != (d->logprob != nullptr)) return KX_EINVAL;
   if (d->top_n < 0 || d->top_n > KX_LOGPROBS_TOP_MAX || d->top_n > d->vocab) return KX_EINVAL;
   if (d->top_n > 0 && (!d->top_ids || !d->top_logprobs)) return KX_EINVAL;
+  if (!aligned4(d->tokens) || !aligned4(d->logprob) || !aligned4(d->entropy) || !aligned4(d->top_ids) || !aligned4(d->top_logprobs))
+    return KX_EINVAL;
   if (!d->workspace || d->workspace_bytes < kx_token_logprobs_workspace_bytes(d->rows, d->vocab, d->top_n)) return KX_EWORKSPACE;
   if ((uintptr_t)d->workspace % 256) return KX_EINVAL;
   if (!grid_fits(d->rows, kLpThreads) || d->vocab > kMostPositions) return KX_ELIMIT;

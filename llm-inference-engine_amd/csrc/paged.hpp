@@ -89,12 +89,13 @@ inline bool stride_ok(int64_t stride, int64_t least, size_t unit) {
   return stride >= least && stride % (int64_t)unit == 0;
 }
 inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+inline bool aligned4(const void* p) { return (uintptr_t)p % 4 == 0; }
 
 inline int paged_check(const kx_paged_kv& d) {
   if (!kind_known(d.type) || d.kv_head_num <= 0 || d.page_size <= 0 || d.num_pages <= 0 || d.table_pages <= 0)
     return KX_EINVAL;
   if (!d.key || !d.value || !d.table || !d.seq_lens || !aligned16(d.key) || !aligned16(d.value)) return KX_EINVAL;
-  if ((uintptr_t)d.table % 4 || (uintptr_t)d.seq_lens % 4) return KX_EINVAL;
+  if (!aligned4(d.table) || !aligned4(d.seq_lens)) return KX_EINVAL;
   if (!head_size_known(d.head_size)) return KX_EUNSUPPORTED;
   const size_t unit = 16 / kind_bytes(d.type);
   if (!stride_ok(d.page_stride, d.head_size, unit) || !stride_ok(d.row_stride, d.head_size, unit) ||

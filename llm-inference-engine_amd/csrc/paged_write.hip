@@ -177,11 +177,12 @@ extern "C" int kx_paged_write(const kx_paged_write_desc* d, void* stream) {
   if (d->rows < 0 || d->kv.batch < 0) return KX_EINVAL;
   if (d->rows == 0 || d->kv.batch == 0) return KX_OK;
   if (const int rc = paged_check(d->kv)) return rc;
-  if (!kind_known(d->src_type) || !d->cu_rows || (uintptr_t)d->cu_rows % 4 || !d->k || !d->v) return KX_EINVAL;
+  if (!kind_known(d->src_type) || !d->cu_rows || !aligned4(d->cu_rows) || !d->k || !d->v) return KX_EINVAL;
   if (!kinds_fit(d->src_type, d->kv.type)) return KX_EUNSUPPORTED;
   if (d->rope_variant != KX_ROPE_INTERLEAVED && d->rope_variant != KX_ROPE_HALF_SPLIT) return KX_EINVAL;
   const bool rope = d->sin_cache != nullptr;
-  if (rope != (d->cos_cache != nullptr) || (rope && d->table_rows <= 0)) return KX_EINVAL;
+  if (rope != (d->cos_cache != nullptr) || (rope && d->table_rows <= 0) || !aligned4(d->sin_cache) || !aligned4(d->cos_cache))
+    return KX_EINVAL;
   if ((d->q != nullptr) != (d->q_out != nullptr) || (d->q && (!rope || d->head_num <= 0))) return KX_EINVAL;
   const int64_t kv_dim = (int64_t)d->kv.kv_head_num * d->kv.head_size, q_dim = (int64_t)d->head_num * d->kv.head_size;
   const size_t unit = 16 / kind_bytes(d->src_type);

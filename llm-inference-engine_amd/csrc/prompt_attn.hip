@@ -658,7 +658,7 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
   if (d->window < 0 || (d->window > 0 && !d->causal) || !isfinite(d->scale)) return KX_EINVAL;
   const int64_t q_dim = (int64_t)d->head_num * d->head_size, kv_dim = (int64_t)d->kv_head_num * d->head_size;
   const size_t bytes = kind_bytes(d->type), unit = 16 / bytes;
-  if (!d->q || !d->out || !d->cu_q || (uintptr_t)d->cu_q % 4 || !aligned16(d->q) || !aligned16(d->out) ||
+  if (!d->q || !d->out || !d->cu_q || !aligned4(d->cu_q) || !aligned16(d->q) || !aligned16(d->out) ||
       !stride_ok(d->q_stride, q_dim, unit) || !stride_ok(d->out_stride, q_dim, unit))
     return KX_EINVAL;
   PromptArgs a{};
@@ -675,7 +675,7 @@ extern "C" int kx_prompt_attention(const kx_prompt_attn_desc* d, void* stream) {
     a.k = a.kv.key;
     a.v = a.kv.value;
   } else {
-    if (!d->k || !d->v || !d->cu_k || (uintptr_t)d->cu_k % 4 || d->k_rows < 0 || !aligned16(d->k) || !aligned16(d->v) ||
+    if (!d->k || !d->v || !d->cu_k || !aligned4(d->cu_k) || d->k_rows < 0 || !aligned16(d->k) || !aligned16(d->v) ||
         !stride_ok(d->k_stride, kv_dim, unit) || !stride_ok(d->v_stride, kv_dim, unit))
       return KX_EINVAL;
     // the rows of a buffer (256 keys at most) are addressed by 31-bit offsets from the first one

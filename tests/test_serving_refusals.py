@@ -70,6 +70,7 @@ def test_pages(bad, code):
     (dict(q_stride=252), EINVAL), (dict(q_out_stride=258), EINVAL), (dict(q=P + 8), EINVAL), (dict(q_out=P + 8), EINVAL), (dict(head_num=0), EINVAL),
     (dict(sin_cache=None), EINVAL), (dict(cos_cache=None), EINVAL), (dict(sin_cache=None, cos_cache=None), EINVAL),
     (dict(table_rows=0), EINVAL), (dict(rope_variant=2), EINVAL), (dict(q_out_stride=264), EINVAL), (dict(rows=1 << 25), ELIMIT),
+    (dict(sin_cache=P + 2), EINVAL), (dict(cos_cache=P + 2), EINVAL),
     (dict(head_num=1 << 24, q_stride=1 << 30, q_out_stride=1 << 30), ELIMIT)])
 def test_write(bad, code):
     assert write(**bad) == code
@@ -122,7 +123,8 @@ def test_prompt_over_pages(bad, code):
     (dict(logits=None), EINVAL), (dict(logits=P + 2), EINVAL), (dict(tokens=None), EINVAL), (dict(logprob=None), EINVAL),
     (dict(top_n=-1), EINVAL), (dict(top_n=33), EINVAL), (dict(top_n=6, vocab=5), EINVAL), (dict(top_ids=None), EINVAL),
     (dict(top_logprobs=None), EINVAL), (dict(workspace=None), EWORKSPACE), (dict(workspace=P + 8), EINVAL),
-    (dict(workspace_bytes=16), EWORKSPACE), (dict(rows=1 << 24), ELIMIT),
+    (dict(workspace_bytes=16), EWORKSPACE), (dict(rows=1 << 24), ELIMIT), (dict(tokens=P + 2), EINVAL),
+    (dict(logprob=P + 1), EINVAL), (dict(entropy=P + 2), EINVAL), (dict(top_ids=P + 2), EINVAL), (dict(top_logprobs=P + 3), EINVAL),
     (dict(vocab=0x7FFFFF01, row_stride=0x7FFFFF01), ELIMIT)])
 def test_logprobs(bad, code):
     assert logprobs(**bad) == code
