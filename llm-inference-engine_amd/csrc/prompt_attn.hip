@@ -38,7 +38,6 @@ namespace kx {
 
 enum PromptOperand { PP_Q, PP_K, PP_V, PP_OUT, PP_CUQ, PP_CUK, PP_TABLE, PP_LENS };
 
-constexpr int kPaWaves = 8;  // waves of a workgroup
 // keys per tile: as many as let two buffers of a tile per group of waves fit LDS
 template <typename T> __host__ __device__ constexpr int pa_keys() { return sizeof(T) == 4 ? 32 : 64; }
 
@@ -156,11 +155,11 @@ template <> struct PromptMma<__bf16> {
 };
 template <> struct PromptMma<float> { typedef f32x4 frag; };
 
-// KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
+// NW: waves of the workgroup.  KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
 // chains of tiles and more workgroups where there are few pairs.
-template <typename T, int HS, int MODE, int KG>
-__global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const PromptArgs a) {
-  constexpr int NW = kPaWaves, PW = NW / KG;     // waves, those of a group
+template <typename T, int HS, int MODE, int KG, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const PromptArgs a) {
+  constexpr int PW = NW / KG;                    // waves of a group
   constexpr int PAIRS = PW * 32;                 // pairs of the workgroup
   constexpr int KT = pa_keys<T>();
   constexpr bool F32 = sizeof(T) == 4, PAGED = MODE != PA_PACKED;
@@ -599,30 +598,30 @@ __global__ __launch_bounds__(kPaWaves * 64, 2) void prompt_attn_kernel(const Pro
 }
 
 // the two buffers; the rows of the results pass through the same place
-template <typename T, int HS, int KG>
+template <typename T, int HS, int KG, int NW>
 constexpr int prompt_lds() {
-  const int row = HS * (int)sizeof(T), tiles = 2 * KG * 2 * pa_keys<T>() * row, rows = KG == 1 ? kPaWaves * 32 * row : 0;
+  const int row = HS * (int)sizeof(T), tiles = 2 * KG * 2 * pa_keys<T>() * row, rows = KG == 1 ? NW * 32 * row : 0;
   return tiles > rows ? tiles : rows;
 }
 
-template <typename T, int HS, int MODE, int KG>
+template <typename T, int HS, int MODE, int KG, int NW>
 static int prompt_launch(const PromptArgs& a, hipStream_t s) {
-  constexpr int pairs = kPaWaves / KG * 32, lds = prompt_lds<T, HS, KG>();
+  constexpr int pairs = NW / KG * 32, lds = prompt_lds<T, HS, KG, NW>();
   // blocks of the sequences: an even share of all pairs and one more each
   const int64_t items = (int64_t)a.q_rows * a.kv_mul / pairs + a.batch;
-  if (!grid_fits(items * a.kv_heads, kPaWaves * 64)) return KX_ELIMIT;
+  if (!grid_fits(items * a.kv_heads, NW * 64)) return KX_ELIMIT;
   static OncePerDevice limit;
   if (lds > 32768)
-    if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, KG>), lds)) return rc;
-  hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, KG>), dim3((unsigned)(items * a.kv_heads)), dim3(kPaWaves * 64), lds, s, a);
+    if (const int rc = limit.raise(reinterpret_cast<const void*>(&prompt_attn_kernel<T, HS, MODE, KG, NW>), lds)) return rc;
+  hipLaunchKernelGGL((prompt_attn_kernel<T, HS, MODE, KG, NW>), dim3((unsigned)(items * a.kv_heads)), dim3(NW * 64), lds, s, a);
   KX_LAUNCH_CHECK();
   return KX_OK;
 }
-template <typename T, int HS, int KG>
+template <typename T, int HS, int KG, int NW>
 static int prompt_mode(const PromptArgs& a, hipStream_t s) {
-  if (!a.kv.table) return prompt_launch<T, HS, PA_PACKED, KG>(a, s);
-  if (a.kv.div.size % 16 == 0) return prompt_launch<T, HS, PA_BLOCK_PAGES, KG>(a, s);
-  return prompt_launch<T, HS, PA_ANY_PAGES, KG>(a, s);
+  if (!a.kv.table) return prompt_launch<T, HS, PA_PACKED, KG, NW>(a, s);
+  if (a.kv.div.size % 16 == 0) return prompt_launch<T, HS, PA_BLOCK_PAGES, KG, NW>(a, s);
+  return prompt_launch<T, HS, PA_ANY_PAGES, KG, NW>(a, s);
 }
 // Groups of waves per workgroup.  Two or more cut a sequence's chain of tiles and give that many times the workgroups, for
 // as many times the K/V traffic per product.
@@ -632,14 +631,21 @@ static int prompt_mode(const PromptArgs& a, hipStream_t s) {
 //   37.9 (8 prompts), 375: 95.6 / 102, 512 (a prompt of 4096): 143 / 155; 64 wide, 85: 11.0 / 9.1, 473: 36.3 / 30.4, 512: 97.2 /
 //   87.7, 1090: 88.2 / 93.2, 2085: 134 / 151; 32 wide, 74: 34.4 / 20.2, 512: 76.9 / 63.0, 674: 51.7 / 57.8.
 //   fp32: as many groups as LDS holds buffers for, always: its products take sixteen times as long and hide the traffic
-//   (64 wide, blocks 31: one 33.7, two 26.8, four 18.9; 612: one 367, four 303; 128 wide, 512: one 1145, two 1097).
+//   (64 wide, blocks 31: one 33.7, two 26.8, four 18.9; 612: one 367, four 303; 128 wide, 512: one 1145, two 1097).  Four waves
+//   instead of eight, one per SIMD, where that many more workgroups still find CUs of their own, or nearly: the chain of
+//   products of a SIMD is half as long.  Measured (us, eight / four, by the workgroups that eight would take): 128 wide, 23:
+//   54.7 / 35.2, 136: 60.2 / 42.1, 280: 49.0 / 38.0, 560: 58.2 / 70.9; 64 wide, 84: 17.3 / 14.4, 180: 27.6 / 20.9, 232: 18.2 /
+//   19.4, 384: 76.7 / 96.6; 32 wide, 52: 11.3 / 9.8, 138: 42.7 / 32.8, 348: 51.0 /
+//   47.1, 650: 26.3 / 33.8.  (16-bit types: nothing, 26.6 / 25.0 at best.)
 template <typename T, int HS>
 static int prompt_groups(const PromptArgs& a, hipStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    return prompt_mode<T, HS, prompt_lds<T, HS, 4>() <= 131072 ? 4 : 2>(a, s);
+    constexpr int KG = prompt_lds<T, HS, 4, 8>() <= 131072 ? 4 : 2;
+    const int64_t workgroups = ((int64_t)a.q_rows * a.kv_mul / (8 / KG * 32) + a.batch) * a.kv_heads;  // of eight waves
+    return workgroups <= (HS == 64 ? 200 : HS == 32 ? 400 : 320) ? prompt_mode<T, HS, KG, 4>(a, s) : prompt_mode<T, HS, KG, 8>(a, s);
   } else {
     const double blocks = (double)a.q_rows * a.kv_mul / 256 * a.kv_heads;
-    return blocks < (HS == 128 ? 320 : HS == 64 ? 800 : 600) ? prompt_mode<T, HS, 2>(a, s) : prompt_mode<T, HS, 1>(a, s);
+    return blocks < (HS == 128 ? 320 : HS == 64 ? 800 : 600) ? prompt_mode<T, HS, 2, 8>(a, s) : prompt_mode<T, HS, 1, 8>(a, s);
   }
 }
 template <typename T>

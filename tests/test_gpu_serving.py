@@ -458,6 +458,20 @@ def test_prompts_over_pages(kind, heads, kv_heads, hs, page, window, head_major)
     check_prompt(q, cu, cache.k, cache.v, got, kind, 1 / np.sqrt(hs), True, window)
 
 
+@pytest.mark.parametrize("hs", [32, 64, 128])
+def test_prompts_of_many_heads(hs):
+    """fp32 calls that fill the chip (others are cut into smaller workgroups): packed rows, pages of whole blocks and others."""
+    rng = np.random.default_rng(hs + 5)
+    heads, lens = 24, [1, 40, 33, 2, 64, 65, 31, 90, 17, 100, 129]
+    cu = np.cumsum([0] + lens)
+    q = rng.standard_normal((cu[-1], heads, hs)).astype(np.float32)
+    for page in (16, 5):
+        cache = Cache(rng, lens, heads, hs, page, kx.F32)
+        got = kx.prompt_attention(q, cu, pool=cache.pool, table=cache.table, seq_lens=lens, kind=kx.F32)
+        check_prompt(q, cu, cache.k, cache.v, got, kx.F32, 1 / np.sqrt(hs))
+    np.testing.assert_array_equal(kx.prompt_attention(q, cu, np.concatenate(cache.k), np.concatenate(cache.v), kind=kx.F32), got)
+
+
 @pytest.mark.parametrize("kind", [kx.F32, kx.F16, kx.BF16], ids=lambda k: NAMES[k])
 @pytest.mark.parametrize("page", [16, 6])
 def test_prompts_missing_pages(kind, page):
