@@ -684,7 +684,9 @@ int kx_paged_decode(const kx_paged_decode_desc* desc, void* stream);
  * p = (keys - n) + i; causal: it sees the keys t <= p, with window > 0 (causal only) of these t > p - window.
  * A row that sees nothing gets zeros; rows of no sequence are left alone.  All of one type
  * (KX_F16 / KX_BF16: matrix-core products of that type with fp32 sums and softmax, probabilities
- * rounded to it for the second product; KX_F32: fp32 throughout).  head_size 32, 64 or 128.  Strides in elements (q and
+ * rounded to it for the second product and for their sum, so that a result lies among the values that it is a mean of;
+ * KX_F32: fp32 throughout).  (As in decode, an infinity among the seen keys and values may give NaN, and a sum of weighted
+ * values that passes the range of fp32 an infinity.)  head_size 32, 64 or 128.  Strides in elements (q and
  * out: head_num * head_size or more, k and v: kv_head_num * head_size or more), multiples of 16 bytes; pointers aligned
  * to 16 bytes; scale finite.  KX_EUNSUPPORTED for packed k or v rows 8 MiB or more apart, pages 4 GiB or more
  * apart or rows of a page 128 MiB or more apart; KX_ELIMIT for 2^31 - 65536 pairs of a row and a head of one kv head, 2^31 - 256

@@ -1,0 +1,106 @@
+"""Batched serving on the GPU at the ends of its ranges: values at the limits of their type, against 64 bits.
+
+Tolerances count U = 2^-24, half a step of fp32, and E(kind), that of a type (see test_gpu_serving)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+import kx  # noqa: E402
+
+from test_gpu_serving import NAMES, U, Cache, rounded  # noqa: E402
+
+TYPES = [kx.F32, kx.F16, kx.BF16]
+
+
+# ------------------------------------------------------------------ a weighted mean is a mean
+def equal_columns(rng, n, kv_heads, hs, kind):
+    """Values that are alike in all rows: the largest of fp16 with both signs, or any."""
+    row = np.where(np.arange(kv_heads * hs) % 2, -1.0, 1.0) * 65504 if kind == kx.F16 else rng.standard_normal(kv_heads * hs)
+    return np.broadcast_to(rounded(row.astype(np.float32), kind).reshape(1, kv_heads, hs), (n, kv_heads, hs)).copy()
+
+
+def assert_means(got, v, g, kind, keys):
+    """got [rows][heads][hs] of rows that see something, v [rows][kv_heads][hs] alike in all rows.  The weights that are
+    summed are those that multiply the values, so the quotient of both sums is off by their roundings alone, 8 sqrt(keys) U
+    of the value: nothing that a 16-bit type shows (half a step is 2^-9 or 2^-12 at least)."""
+    want = np.repeat(v[:1], g, axis=1)
+    if kind == kx.F32:
+        assert (np.abs(got - want) <= (8 * np.sqrt(keys) * U + 2.0 ** -20) * np.abs(want)).all()
+    else:
+        np.testing.assert_array_equal(got, np.broadcast_to(want, got.shape))
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("paged", [False, True])
+def test_prompt_means_of_equal_values(kind, hs, paged):
+    rng = np.random.default_rng(hs + kind)
+    n, heads, kv_heads = 460, 6, 2
+    cache = Cache(rng, [n], kv_heads, hs, 16, kind)
+    q = rounded(rng.standard_normal((n, heads, hs)).astype(np.float32) * 4, kind)  # few keys carry most of the weight
+    k, v = cache.k[0], equal_columns(rng, n, kv_heads, hs, kind)
+    if paged:
+        pool = kx.PagePool(*(a[np.arange(480) % n].reshape(30, 16, kv_heads, hs) for a in (k, v)), kind)
+        table = np.arange(30, dtype=np.int32)[None]
+        got = kx.prompt_attention(q, [0, n], pool=pool, table=table, seq_lens=[n], kind=kind)
+        one = kx.paged_decode(pool, table, [n], q[-1:], q_kind=kind)
+        assert_means(one, v, 3, kind, n)
+    else:
+        got = kx.prompt_attention(q, [0, n], k, v, kind=kind)
+    assert_means(got, v, 3, kind, n)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+def test_prompt_mean_with_one_key_far_above_the_first(kind):
+    """One key at score zero in the first tile and one 256 keys on (in a later tile of the same waves), 6 to 8 powers of two
+    above it, nearly alone with each other: the running maximum stays with the first, so the second one's weight is among
+    the largest that are held."""
+    rng = np.random.default_rng(7)
+    rows, keys, hs = 256, 300, 64
+    q = np.zeros((rows, 1, hs), np.float32)
+    q[:, 0, 0] = np.linspace(6, 8, rows) * np.log(2)
+    q[:, 0, 1] = 1
+    k = np.zeros((keys, 1, hs), np.float32)
+    k[:, 0, 1] = -60
+    k[[0, 262], 0, 1] = 0
+    k[262, 0, 0] = 1
+    q, k, v = rounded(q, kind), rounded(k, kind), equal_columns(rng, keys, 1, hs, kind)
+    got = kx.prompt_attention(q, [0, rows], k, v, cu_k=[0, keys], causal=False, scale=1.0, kind=kind)
+    assert_means(got, v, 1, kind, keys)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+def test_prompt_mean_of_a_strong_key_and_many_weak_ones(kind):
+    """20 000 keys of 2^-22 of the weight of one: they are half a percent of the sum, though each is next to nothing."""
+    rng = np.random.default_rng(8)
+    rows, keys, hs = 3, 20000, 32
+    q, k = np.zeros((rows, 1, hs), np.float32), np.zeros((keys, 1, hs), np.float32)
+    q[:, 0, 0] = 1
+    k[:, 0, 0] = np.where(np.arange(keys) == 11, 15.25, 0)  # 15.25 = 22 ln 2
+    v = np.full((keys, 1, hs), 3.0, np.float32)
+    v[11] = 1.0
+    got = kx.prompt_attention(q, [0, rows], k, v, cu_k=[0, keys], causal=False, scale=1.0, kind=kind)
+    w = np.exp(-15.25) * (keys - 1)
+    want = (1 + 3 * w) / (1 + w)
+    # the weak weights round to a type by half a step of it at most (fp16 holds them with 2^-10 there)
+    relative = {kx.F32: 2.0 ** -18, kx.F16: 2.0 ** -10, kx.BF16: 2.0 ** -8}[kind] * w * 3
+    half = {kx.F32: U, kx.F16: 2.0 ** -11, kx.BF16: 2.0 ** -8}[kind] * want
+    assert (np.abs(got - want) <= relative + half + 8 * np.sqrt(keys) * U * want).all()
+    v[:] = equal_columns(rng, 1, 1, hs, kx.BF16) if kind == kx.BF16 else 1000.0
+    got = kx.prompt_attention(q, [0, rows], k, v, cu_k=[0, keys], causal=False, scale=1.0, kind=kind)
+    assert_means(got, v, 1, kind, keys)
+
+
+@pytest.mark.parametrize("kind", [kx.F16, kx.BF16], ids=lambda k: NAMES[k])
+def test_prompt_means_beside_hidden_nan_and_seen_infinity(kind):
+    """Rows ahead of a NaN are computed from what they see alone; an infinity that is seen stays one."""
+    rng = np.random.default_rng(9)
+    n, hs = 200, 64
+    q, k = (rounded(rng.standard_normal((n, m, hs)).astype(np.float32), kind) for m in (4, 2))
+    v = equal_columns(rng, n, 2, hs, kind)
+    want = v.copy()
+    v[190, :, 3], v[193, :, 5], v[195] = np.inf, -np.inf, np.nan
+    got = kx.prompt_attention(q, [0, n], k, v, kind=kind)
+    assert_means(got[:190], want, 2, kind, n)
+    assert np.isposinf(got[190:195, :, 3]).all() and np.isneginf(got[193:195, :, 5]).all() and np.isnan(got[195:]).all()
