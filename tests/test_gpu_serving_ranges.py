@@ -104,3 +104,38 @@ def test_prompt_means_beside_hidden_nan_and_seen_infinity(kind):
     got = kx.prompt_attention(q, [0, n], k, v, kind=kind)
     assert_means(got[:190], want, 2, kind, n)
     assert np.isposinf(got[190:195, :, 3]).all() and np.isneginf(got[193:195, :, 5]).all() and np.isnan(got[195:]).all()
+
+
+# ------------------------------------------------------------------ sure tokens
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("rows,vocab", [(3, 40000), (64, 128256), (1100, 20000), (2, 37)])
+def test_logprobs_of_sure_tokens(kind, rows, vocab):
+    """Three logits that are not banned: one at the start, one further on and the likeliest behind both, up to 17 above the
+    first.  No probability passes one and no entropy falls below zero, and both hold to the last bits:
+    relative to the largest logit, d = x - max rounds to U |d|, e^d to U (2 |d| + 4) of itself, the sum z of 1 and two others
+    to 2 U z, ln z to U (2 + 2 ln z), the last difference to U of its result; a share p of the entropy likewise."""
+    rng = np.random.default_rng(rows + vocab)
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    at = np.array([0, 5, 20]) if vocab < 100 else np.array([1, vocab // 3, vocab - 7])
+    gap = rng.uniform(0.5, 17, (rows, 2)).astype(np.float32)
+    x[:, at[2]] = rng.uniform(-4, 4, rows)
+    x[:, at[0]], x[:, at[1]] = x[:, at[2]] - gap[:, 0], x[:, at[2]] - gap[:, 1]
+    x[0, at] = [-3.0, -12.75, 12.875]
+    x = rounded(x, kind)
+    order = np.argsort(-x[:, at].astype(np.float64), axis=1, kind="stable")
+    lp, en, ids, tl = kx.token_logprobs(x, np.full(rows, at[2]), 3, kind)
+    np.testing.assert_array_equal(ids, at[order])
+    d = x[:, at].astype(np.float64)
+    d -= d.max(1, keepdims=True)
+    z = np.exp(d).sum(1)
+    off_e = np.exp(d) * U * (2 * np.abs(d) + 4)
+    off_lz = off_e.sum(1) / z + 2 * U + U * (2 + 2 * np.log(z))
+    want = d - np.log(z)[:, None]
+    off = off_lz[:, None] + U * np.abs(d) + U * np.abs(want)
+    assert (tl <= 0).all() and (lp <= 0).all()
+    assert (np.abs(tl - np.take_along_axis(want, order, 1)) <= np.take_along_axis(off, order, 1)).all()
+    assert (np.abs(lp - want[:, 2]) <= off[:, 2]).all()
+    p = np.exp(want)
+    h = -(p * want).sum(1)
+    off_h = off_lz + (np.exp(d) * np.abs(d) * U * (2 * np.abs(d) + 8)).sum(1) / z + 4 * U * h
+    assert (en >= 0).all() and (np.abs(en - h) <= off_h).all()
