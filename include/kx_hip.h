@@ -690,7 +690,8 @@ int kx_paged_decode(const kx_paged_decode_desc* desc, void* stream);
  * out: head_num * head_size or more, k and v: kv_head_num * head_size or more), multiples of 16 bytes; pointers aligned
  * to 16 bytes; scale finite.  KX_EUNSUPPORTED for packed k or v rows 8 MiB or more apart, pages 4 GiB or more
  * apart or rows of a page 128 MiB or more apart; KX_ELIMIT for 2^31 - 65536 pairs of a row and a head of one kv head, 2^31 - 256
- * key rows, or more than 2^23 workgroups (a workgroup has 64 such pairs or more, a sequence one workgroup per kv head or more). */
+ * key rows, or 2^23 workgroups and more (each has 64 such pairs or more, a sequence one workgroup per kv head or more; fp32
+ * calls of a few hundred workgroups take smaller ones, of 32 pairs or more, and are far from that limit). */
 typedef struct kx_prompt_attn_desc {
   int32_t type;
   int32_t head_num, kv_head_num, head_size;
