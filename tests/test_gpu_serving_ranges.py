@@ -1,4 +1,5 @@
-"""Batched serving on the GPU at the ends of its ranges: values at the limits of their type, against 64 bits.
+"""Batched serving on the GPU at the ends of its ranges: values at the limits of their type, batches of more sequences than
+a wave has lanes, prompts that fill the chip, against 64 bits.
 
 Tolerances count U = 2^-24, half a step of fp32, and E(kind), that of a type (see test_gpu_serving)."""
 import numpy as np
@@ -8,7 +9,8 @@ pytestmark = pytest.mark.gpu
 
 import kx  # noqa: E402
 
-from test_gpu_serving import NAMES, U, Cache, rounded  # noqa: E402
+from test_gpu_serving import (E, KINDS, NAMES, U, Cache, check_decode, check_prompt, close, exact_attention,  # noqa: E402
+                              exact_rope, rope_tables, rounded)
 
 TYPES = [kx.F32, kx.F16, kx.BF16]
 
@@ -139,3 +141,152 @@ def test_logprobs_of_sure_tokens(kind, rows, vocab):
     h = -(p * want).sum(1)
     off_h = off_lz + (np.exp(d) * np.abs(d) * U * (2 * np.abs(d) + 8)).sum(1) / z + 4 * U * h
     assert (en >= 0).all() and (np.abs(en - h) <= off_h).all()
+
+
+# ------------------------------------------------------------------ more sequences than a wave has lanes
+BATCHES = [63, 64, 65, 129, 200]
+
+
+def ragged(rng, batch, most):
+    """Lengths of 0 .. most, with sequences of none and of one on both sides of every 64th."""
+    n = rng.integers(0, most + 1, batch)
+    for edge in range(64, batch + 1, 64):
+        for i, at in enumerate(range(edge - 2, min(edge + 2, batch))):
+            n[at] = (0, 1, 0, 2)[(i + edge // 64) % 4]
+    n[-1] = most
+    return n
+
+
+@pytest.mark.parametrize("batch", BATCHES + [4096, 4097, 4300])
+@pytest.mark.parametrize("src,kind", [(kx.F32, kx.F16), (kx.BF16, kx.BF16)], ids=lambda k: NAMES[k])
+def test_write_many_sequences(src, kind, batch):
+    rng = np.random.default_rng(batch)
+    hs, page, variant = 32, 4, batch % 2
+    new = ragged(rng, batch, 5)
+    lens = new + rng.integers(0, 9, batch)
+    held = -(-lens // page)
+    pages = rng.permutation(held.sum() + 2)
+    table = np.full((batch, held.max()), -1, np.int32)
+    table[np.arange(held.max())[None] < held[:, None]] = pages[:held.sum()]
+    key = np.full((len(pages), page, 1, hs), np.nan, np.float32)
+    pool = kx.PagePool(key, key, kind)
+    cu = 1 + np.concatenate([[0], np.cumsum(new)])
+    rows = cu[-1] + 2
+    q, k, v = (rounded(rng.standard_normal((rows, n, hs)).astype(np.float32), src) for n in (2, 1, 1))
+    tables = rope_tables(16, hs)
+    got_q = kx.paged_write(pool, table, lens, cu, k, v, q, tables, variant, src, in_place=True)
+    got_k, got_v = pool.read()
+    seq = np.repeat(np.arange(batch), new)
+    row = np.arange(cu[0], cu[-1])
+    pos = row - cu[seq + 1] + lens[seq]
+    at = (table[seq, pos // page], pos % page)
+    want_v = key.copy()
+    want_v[at] = rounded(v[row], kind)
+    np.testing.assert_array_equal(got_v, want_v)
+    assert (np.isnan(got_k) == np.isnan(want_v)).all()
+    for x, got, kind_of in ((q, got_q[row], src), (k, got_k[at], kind)):
+        pairs = [exact_rope(x[r], p, tables, variant) for r, p in zip(row, pos)]
+        want, size = np.stack([y for y, _ in pairs]), np.stack([z for _, z in pairs])
+        # two products and a sum in fp32, then the type's rounding, as in test_write
+        assert (np.abs(got - want) <= 3 * U * size + E[kind_of] * np.abs(want) * (1 + 2 ** -7) + (2.0 ** -25 if kind_of == kx.F16 else 0)).all()
+    outside = np.setdiff1d(np.arange(rows), row)
+    np.testing.assert_array_equal(got_q[outside], q[outside])
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("q_kind,kind", KINDS, ids=lambda k: NAMES[k])
+def test_decode_many_sequences(q_kind, kind, batch):
+    """Long sequences, which are cut over workgroups, ahead of the 64th, behind it and at both ends."""
+    rng = np.random.default_rng(batch + kind)
+    lens = ragged(rng, batch, 40)
+    for at in (0, 3, 62, 66, 70, 127, 130, batch - 1):
+        if at < batch:
+            lens[at] = 2000 + 37 * (at % 50)
+    heads, kv_heads, hs, page = [(3, 1, 32, 16), (4, 2, 64, 5)][batch % 2]
+    cache = Cache(rng, lens.tolist(), kv_heads, hs, page, kind)
+    q = rounded(rng.standard_normal((batch, heads, hs)).astype(np.float32), q_kind)
+    got = kx.paged_decode(cache.pool, cache.table, lens, q, q_kind=q_kind)
+    assert (got[lens == 0] == 0).all()
+    check_decode(cache, q, got, 0, 1 / np.sqrt(hs), q_kind)
+    got = kx.paged_decode(cache.pool, cache.table, lens, q, window=1000, q_kind=q_kind)
+    check_decode(cache, q, got, 1000, 1 / np.sqrt(hs), q_kind)
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+def test_prompts_of_many_sequences(kind, batch):
+    rng = np.random.default_rng(batch + kind)
+    heads, kv_heads, hs = [(3, 1, 32), (4, 2, 64)][batch % 2]
+    new = ragged(rng, batch, 20)
+    new[[5, batch // 2]] = 150, 70
+    cu = 2 + np.concatenate([[0], np.cumsum(new)])
+    rows = cu[-1] + 3
+    q, k, v = (rounded(rng.standard_normal((rows, n, hs)).astype(np.float32), kind) for n in (heads, kv_heads, kv_heads))
+    got = kx.prompt_attention(q, cu, k, v, kind=kind, fill=7.0)
+    assert (got[:2] == 7).all() and (got[-3:] == 7).all()
+    check_prompt(q, cu, [k[a:b] for a, b in zip(cu, cu[1:])], [v[a:b] for a, b in zip(cu, cu[1:])], got, kind, 1 / np.sqrt(hs))
+    lens = new + rng.integers(0, 30, batch)
+    for page in (16, 7):
+        cache = Cache(rng, lens.tolist(), kv_heads, hs, page, kind)
+        got = kx.prompt_attention(q, cu, pool=cache.pool, table=cache.table, seq_lens=lens, window=25, kind=kind, fill=7.0)
+        assert (got[:2] == 7).all() and (got[-3:] == 7).all()
+        check_prompt(q, cu, cache.k, cache.v, got, kind, 1 / np.sqrt(hs), window=25)
+
+
+# ------------------------------------------------------------------ prompts that fill the chip
+def check_sample(rng, q, cu, ks, vs, got, kind, scale, window, hidden=None):
+    """A sample of rows and heads against 64 bits; hidden: key positions of each sequence that are not there."""
+    g = q.shape[1] // ks[0].shape[1]
+    for b in range(len(cu) - 1):
+        n, m = cu[b + 1] - cu[b], len(ks[b])
+        if not n:
+            continue
+        sample = np.unique(np.concatenate([[0, n - 1, min(n - 1, 63), min(n - 1, 64)], rng.integers(0, n, 6)]))
+        for h in np.unique(np.concatenate([[0, q.shape[1] - 1], rng.integers(0, q.shape[1], 4)])):
+            at, p = np.arange(m)[None], (m - n + sample)[:, None]
+            seen = at <= p
+            if window:
+                seen &= at > p - window
+            if hidden is not None:
+                seen &= ~hidden[b][None]
+            want, spread, size = exact_attention(q[cu[b] + sample, h], ks[b][:, h // g], vs[b][:, h // g], seen, scale)
+            close(got[cu[b] + sample, h], want, spread, size, E[kind], kind)
+
+
+@pytest.mark.parametrize("kind", [kx.F16, kx.BF16], ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("heads,hs", [(64, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("page", [0, 16, 5])
+def test_prompts_that_fill_the_chip(kind, heads, hs, page):
+    """Enough rows and heads that a workgroup keeps its keys to itself (256 pairs of a row and a head each: 320 such workgroups
+    for 128-wide heads, 800 for 64, 600 for 32): packed rows, pages of whole blocks, others; windows, missing pages, and a NaN
+    in a value that rows ahead of it do not see."""
+    rng = np.random.default_rng(heads + hs + page)
+    kv_heads, scale = 8, hs ** -0.5
+    new = [800, 1, 0, 60, 870]
+    cu = np.cumsum([0] + new)
+    assert cu[-1] * heads / 256 >= {128: 320, 64: 800, 32: 600}[hs]
+    q = rounded(rng.standard_normal((cu[-1], heads, hs)).astype(np.float32), kind)
+    if not page:
+        k, v = (rounded(rng.standard_normal((cu[-1], kv_heads, hs)).astype(np.float32), kind) for _ in range(2))
+        ks, vs = ([a[i:j] for i, j in zip(cu, cu[1:])] for a in (k, v))
+        for window in (0, 100):
+            got = kx.prompt_attention(q, cu, k, v, window=window, kind=kind)
+            check_sample(rng, q, cu, ks, vs, got, kind, scale, window)
+        broken = v.copy()
+        broken[cu[4] - 3] = np.nan  # the third last row of the fourth sequence
+        got = kx.prompt_attention(q, cu, k, broken, kind=kind)
+        assert np.isnan(got[cu[4] - 3:cu[4]]).all() and np.isfinite(got[:cu[4] - 3]).all() and np.isfinite(got[cu[4]:]).all()
+        check_sample(rng, q, [cu[3], cu[4] - 3], [ks[3][:-3]], [vs[3][:-3]], got, kind, scale, 0)
+        return
+    lens = [n + c for n, c in zip(new, [200, 0, 20, 333, 90])]
+    cache = Cache(rng, lens, kv_heads, hs, page, kind)
+    for window in (0, 150):
+        got = kx.prompt_attention(q, cu, pool=cache.pool, table=cache.table, seq_lens=lens, window=window, kind=kind)
+        check_sample(rng, q, cu, cache.k, cache.v, got, kind, scale, window)
+    table = cache.table.copy()
+    hidden = [np.zeros(n, bool) for n in lens]
+    for b, col in ((0, 3), (0, 1000 // page - 1), (3, 0), (4, 20)):
+        table[b, col] = [-1, 1 << 30][col % 2]
+        hidden[b][col * page:(col + 1) * page] = True
+    got = kx.prompt_attention(q, cu, pool=cache.pool, table=table, seq_lens=lens, kind=kind)
+    check_sample(rng, q, cu, cache.k, cache.v, got, kind, scale, 0, hidden)
