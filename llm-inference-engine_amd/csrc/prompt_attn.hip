@@ -29,6 +29,10 @@
 // them.  (With the sum of the unrounded weights, values of 65504 came out as infinity.  Dot products with ones sum them; measured in
 // turn against that, us: a prompt of 4096 143 / 145, packed prompts 52.7 / 52.0, pieces 94.3 / 93.8.)  The running maximum follows only when it is
 // exceeded by more than 2^8: weights up to 256 have the same relative precision, and the rescaling pass is rare.
+//
+// Values that are not finite and that some pairs of a tile do not see: the edge tiles are looked through for them (1 % of a
+// prompt of 4096), and one that holds any is taken key by key when the others are done: 50 - 70 us per wave, side by side.  (Pairs
+// with such a result computed anew over all of their keys, one after the other, took 27 ms for a prompt of 4096.)
 #include <math.h>
 
 #include <type_traits>
@@ -165,10 +169,27 @@ template <> struct PromptMma<__bf16> {
 };
 template <> struct PromptMma<float> { typedef f32x4 frag; };
 
+// c and the products of the elements of two dwords
+template <typename T>
+__device__ __forceinline__ float dot_dword(unsigned x, unsigned y, float c) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaf(__uint_as_float(x), __uint_as_float(y), c);
+  } else if constexpr (std::is_same<T, _Float16>::value) {
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, x), __builtin_bit_cast(pair, y), c, false);
+  } else {
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, x), __builtin_bit_cast(pair, y), c, false);
+  }
+}
+typedef const __attribute__((address_space(3))) u32x4* lds_vec_ptr;
+__device__ __forceinline__ u32x4 read_tile(lds_vec_ptr __restrict__ p) { return *p; }  // (restrict: as above)
+
 // NW: waves of the workgroup.  KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
-// chains of tiles and more workgroups where there are few pairs.
+// chains of tiles and more workgroups where there are few pairs.  (Narrower heads of 16-bit types keep to 128 registers: two workgroups
+// share a CU.)
 template <typename T, int HS, int MODE, int KG, int NW>
-__global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const PromptArgs a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW / 4) void prompt_attn_kernel(const PromptArgs a) {
   constexpr int PW = NW / KG;                    // waves of a group
   constexpr int PAIRS = PW * 32;                 // pairs of the workgroup
   constexpr int KT = pa_keys<T>();
@@ -336,6 +357,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
   float m = -INFINITY, l = 0.f;  // m in units of the raw product
+  int odd_first = 0, odd_last = -1;  // first key of the first and of the last tile that is left for the end
 
   bool missing = false;
   if (PAGED && t0 < t1) {
@@ -397,20 +419,49 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
         if (more) issue(t + KG, buf ^ 1, kt * RP / HALVES, (kt + 1) * RP / HALVES);
       }
       if (t + 2 * KG < t1) get_ids(t + 2 * KG);
+      bool odd = false;
       if (key0 + KT > full_hi || key0 < full_lo || missing) {
-        unsigned long long there = ~0ull;
-        if (PAGED && missing) {
+        // keys of the tile that are there
+        auto pages_there = [&]() {
           const int at = key0 + lane;
-          there = __ballot(at < w.keys && page_ok(lookup(min(at, w.keys - 1))));
-        }
-        there >>= 4 * half;
+          return __ballot(at < w.keys && page_ok(lookup(min(at, w.keys - 1))));
+        };
+        unsigned long long there = PAGED && missing ? pages_there() : ~0ull;
+        const unsigned long long mine = there >> 4 * half;
 #pragma unroll
         for (int kt = 0; kt < KT / 32; ++kt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int k = 32 * kt + 8 * (r / 4) + r % 4, at = key0 + k + 4 * half;
-            if (at >= my_hi || at < my_lo || !(there >> k & 1)) s[kt][r] = -INFINITY;
+            if (at >= my_hi || at < my_lo || !(mine >> k & 1)) s[kt][r] = -INFINITY;
           }
+        // A value that is not finite must not meet the weight of zero of a pair that does not see it: a tile with such is left
+        // for the end.  Values of pages that are not there become zeros instead (every wave that finds some writes these
+        // ahead of its own reads; no pair sees them).
+        auto look = [&]() {
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};  // 0, or NaN (0 times what is not finite)
+#pragma unroll 4
+          for (int j = 0; j < KP; ++j) {
+            const u32x4 x = read_tile((lds_vec_ptr)(base + TILEB + j * 1024 + lane * 16));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[e] = dot_dword<T>(x[e], 0u, sums[e]);
+          }
+          return __ballot(sums[0] + sums[1] + sums[2] + sums[3] != 0.f) != 0;
+        };
+        odd = look();
+        if (PAGED && odd) {
+          if (!missing) there = pages_there();
+#pragma unroll 1
+          for (int j = 0; j < KP; ++j)
+            if (!(there >> (j * RPP + lane / CH) & 1))
+              *(__attribute__((address_space(3))) u32x4*)(base + TILEB + j * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          odd = look();
+        }
+        if (odd) {
+          if (odd_last < 0) odd_first = key0;
+          odd_last = key0;
+        }
       }
       float mx = s[0][0];
 #pragma unroll
@@ -430,41 +481,43 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
         m = m_new;
       }
       const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
+      if (!odd) {
 #pragma unroll
-      for (int kt = 0; kt < KT / 32; ++kt) {
-        float sum = 0.f;
+        for (int kt = 0; kt < KT / 32; ++kt) {
+          float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mc));
-          if constexpr (F32) sum += s[kt][r];
-        }
-        if constexpr (F32) {
+          for (int r = 0; r < 16; ++r) {
+            s[kt][r] = __builtin_amdgcn_exp2f(fmaf(s[kt][r], c, -mc));
+            if constexpr (F32) sum += s[kt][r];
+          }
+          if constexpr (F32) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
+            for (int r = 0; r < 16; ++r)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              const float vf = *(const __attribute__((address_space(3))) float*)(base + vfrag[dt] + (32 * kt + 8 * (r / 4) + r % 4) * ROWB);
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[kt][r], o[dt], 0, 0, 0);
-            }
-        } else {
+              for (int dt = 0; dt < DT; ++dt) {
+                const float vf = *(const __attribute__((address_space(3))) float*)(base + vfrag[dt] + (32 * kt + 8 * (r / 4) + r % 4) * ROWB);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[kt][r], o[dt], 0, 0, 0);
+              }
+          } else {
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            frag pf;
+            for (int st = 0; st < 2; ++st) {
+              frag pf;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) pf[j] = (T)s[kt][8 * st + j];
+              for (int j = 0; j < 8; ++j) pf[j] = (T)s[kt][8 * st + j];
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) sum = PromptMma<T>::add_pair(pf[j], pf[j + 1], sum);
+              for (int j = 0; j < 8; j += 2) sum = PromptMma<T>::add_pair(pf[j], pf[j + 1], sum);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-              const lds_bytes at = base + vfrag[dt] + (32 * kt + 16 * st) * ROWB;
-              const s16x4 lo4 = read_transposed((lds_tr_ptr)at);
-              const s16x4 hi4 = read_transposed((lds_tr_ptr)(at + 8 * ROWB));
-              const s16x8 both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-              o[dt] = PromptMma<T>::mul(__builtin_bit_cast(frag, both), pf, o[dt]);
+              for (int dt = 0; dt < DT; ++dt) {
+                const lds_bytes at = base + vfrag[dt] + (32 * kt + 16 * st) * ROWB;
+                const s16x4 lo4 = read_transposed((lds_tr_ptr)at);
+                const s16x4 hi4 = read_transposed((lds_tr_ptr)(at + 8 * ROWB));
+                const s16x8 both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[dt] = PromptMma<T>::mul(__builtin_bit_cast(frag, both), pf, o[dt]);
+              }
             }
           }
+          l += sum;
         }
-        l += sum;
       }
     } else {
       if (more) issue(t + KG, buf ^ 1, 0, RP);
@@ -472,6 +525,61 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+  }
+  // ---- the tiles that were left: key by key, each pair with those that it sees, from memory.  A lane has half of its pair's
+  //      query and of its values ----
+  for (int key0 = odd_first; key0 <= odd_last; key0 += KG * KT) {
+    if (key0 + KT <= full_hi && key0 >= full_lo && !missing) continue;
+    // a row's byte offset; whether it is there
+    auto row_at = [&](int t, int64_t stride, bool& there) -> int64_t {
+      if constexpr (PAGED) {
+        const int page = lookup(t);
+        there = page_ok(page);
+        return paged_offset(page, t);
+      } else {
+        there = true;
+        return t * stride * (int)sizeof(T);
+      }
+    };
+    float sum = 0.f;
+    for (int j = 0; j < KP; ++j) {
+      const int t = key0 + j * RPP + lane / CH;
+      bool there;
+      const char* vr = reinterpret_cast<const char*>(vbase) + row_at(min(t, w.keys - 1), v_stride, there) + lane % CH * 16;
+      if (t >= w.keys || !there) continue;
+      const u32x4 x = *KX_CK(a, PP_V, reinterpret_cast<const u32x4*>(vr));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum = dot_dword<T>(x[e], 0u, sum);
+    }
+    if (!__ballot(sum != 0.f)) continue;
+    const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
+#pragma unroll 1
+    for (int t = max(key0, w_lo); t < min(key0 + KT, w_hi); ++t) {
+      bool there;
+      const char* kr = reinterpret_cast<const char*>(kbase) + row_at(t, k_stride, there) + 16 * half;
+      const char* vr = reinterpret_cast<const char*>(vbase) + row_at(t, v_stride, there) + 4 * half * (int)sizeof(T);
+      if (!there) continue;
+      float x = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 k4 = *KX_CK(a, PP_K, reinterpret_cast<const u32x4*>(kr + 32 * ks)), q4 = __builtin_bit_cast(u32x4, qf[ks]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = dot_dword<T>(k4[e], q4[e], x);
+      }
+      x += __shfl_xor(x, 32);
+      const bool seen = t >= my_lo && t < my_hi;
+      const float weight = seen ? (float)(T)__builtin_amdgcn_exp2f(fmaf(x, c, -mc)) : 0.f;
+      l += half == 0 ? weight : 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v4[4];
+          load4(KX_CKN(a, PP_V, reinterpret_cast<const T*>(vr) + 32 * dt + 8 * q, 4 * sizeof(T)), v4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = seen ? fmaf(weight, v4[e], o[dt][4 * q + e]) : o[dt][4 * q + e];
+        }
+    }
   }
   l = xor32_sum(l);
   if constexpr (KG > 1) {
@@ -516,7 +624,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
 
   // ---- results: through the wave's part of LDS to whole rows ----
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  float odd = 0.f;  // NaN if any result is not finite
   // (with groups: where the first of the parts that this wave alone has read lies)
   char* region = smem + wave * (KG > 1 ? (DT * 16 + 2) * 256 : 32 * ROWB);
   static_assert((DT * 16 + 2) * 256 >= 32 * ROWB, "");
@@ -529,85 +636,21 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void prompt_attn_kernel(const Prom
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = o[dt][4 * q + e] * inv;
-        odd = fmaf(x, 0.f, odd);
-        y[e] = round_to<T>(x);
+        y[e] = fabsf(x) < INFINITY ? round_to<T>(x) : (T)x;  // (an infinity that is seen stays one)
       }
       const int byte = (32 * dt + 8 * q + 4 * half) * (int)sizeof(T);
       *reinterpret_cast<vec*>(region + qcol * ROWB + ((byte >> 4 ^ k_swizzle<CH>(qcol)) << 4) + (byte & 15)) = y;
     }
-  unsigned long long redo = __ballot(odd != 0.f);
-  const unsigned redo_rows = (unsigned)(redo | redo >> 32);
   // (a wave's LDS instructions are served in order: it reads what its own lanes wrote)
 #pragma unroll
   for (int j = 0; j < 32 / RPP; ++j) {
     const int r = j * RPP + lane / CH, p = lane % CH;
     const u32x4 y = *reinterpret_cast<const u32x4*>(region + r * ROWB + ((p ^ k_swizzle<CH>(r)) << 4));
     const int f = wf0 + r;
-    if (f < pairs && !(redo_rows >> r & 1)) {
+    if (f < pairs) {
       const int row = a.mul_div.page(f);
       char* dst = a.out + ((w.q0 + row) * a.out_stride + (kvh * a.kv_mul + f - row * a.kv_mul) * HS) * (int64_t)sizeof(T) + 16 * p;
       *KX_CKN(a, PP_OUT, reinterpret_cast<u32x4*>(dst), 16) = y;
-    }
-  }
-  // A pair whose result is not finite is computed again from the rows that it sees and no others: a NaN or an infinity in a
-  // V row that is hidden from it has met a weight of zero above.  Lanes take a key each for the scores, then a
-  // part of the row each for the sum.
-  for (unsigned left = redo_rows; left; left &= left - 1) {
-    const int f = wf0 + __builtin_ctz(left);
-    if (f >= pairs) break;
-    const int row = a.mul_div.page(f), head = kvh * a.kv_mul + f - row * a.kv_mul;
-    const int r_hi = hi_of(row), r_lo = lo_of(row);
-    auto key_row = [&](const T* base, int64_t stride, int t, bool& there) -> const T* {
-      if constexpr (PAGED) {
-        const int page = lookup(t);
-        there = page_ok(page);
-        return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + paged_offset(page, t));
-      } else {
-        there = true;
-        return base + t * stride;
-      }
-    };
-    const T* qr = reinterpret_cast<const T*>(a.q) + (w.q0 + row) * a.q_stride + head * HS;
-    constexpr int VE = HS >= 64 ? HS / 64 : 1;
-    float rm = -INFINITY, rl = 0.f, acc[VE] = {};
-    const int d0 = min(lane * VE, HS - VE);
-    for (int base = r_lo; base < r_hi; base += 64) {
-      const int t = min(base + lane, r_hi - 1);
-      bool there;
-      const T* kr = key_row(kbase, k_stride, t, there);
-      float x = 0.f;
-      for (int d = 0; d < HS; d += 4) {
-        float k4[4], q4[4];
-        load4(KX_CKN(a, PP_K, kr + d, 4 * sizeof(T)), k4);
-        load4(KX_CKN(a, PP_Q, qr + d, 4 * sizeof(T)), q4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x = fmaf(k4[e], a.scale < 0.f ? -q4[e] : q4[e], x);
-      }
-      if (!there || base + lane >= r_hi) x = -INFINITY;
-      const unsigned long long seen = __ballot(there && base + lane < r_hi);
-      const float nm = fmaxf(rm, wave_max(x));
-      const float alpha = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((rm - nm) * c);
-      const float p = __builtin_amdgcn_exp2f((x - (nm == -INFINITY ? 0.f : nm)) * c);
-      rm = nm;
-      rl = rl * alpha + wave_sum(p);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] *= alpha;
-      for (int j = 0; j < 64 && base + j < r_hi; ++j) {
-        const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
-        if (!(seen >> j & 1)) continue;
-        bool ok;
-        const T* vr = key_row(vbase, v_stride, base + j, ok) + d0;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) acc[e] = fmaf(pj, (float)*KX_CK(a, PP_V, vr + e), acc[e]);
-      }
-    }
-    if (lane * VE < HS) {
-      T* dst = reinterpret_cast<T*>(a.out) + (w.q0 + row) * a.out_stride + head * HS + d0;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float x = rl == 0.f ? 0.f : acc[e] / rl;
-        *KX_CK(a, PP_OUT, dst + e) = fabsf(x) < INFINITY ? round_to<T>(x) : (T)x;  // (an infinity that is seen stays one)
-      }
     }
   }
 }

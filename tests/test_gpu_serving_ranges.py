@@ -2,6 +2,9 @@
 a wave has lanes, prompts that fill the chip, against 64 bits.
 
 Tolerances count U = 2^-24, half a step of fp32, and E(kind), that of a type (see test_gpu_serving)."""
+import ctypes as C
+import time
+
 import numpy as np
 import pytest
 
@@ -106,6 +109,111 @@ def test_prompt_means_beside_hidden_nan_and_seen_infinity(kind):
     got = kx.prompt_attention(q, [0, n], k, v, kind=kind)
     assert_means(got[:190], want, 2, kind, n)
     assert np.isposinf(got[190:195, :, 3]).all() and np.isneginf(got[193:195, :, 5]).all() and np.isnan(got[195:]).all()
+
+
+# ------------------------------------------------------------------ values that are not finite
+def check_around(q, cu, ks, vs, got, kind, scale, window, first, broken):
+    """broken: (sequence, key, column, value) of values that are not finite in vs; `first`: the sequences' first key that is
+    there.  Rows that see one have it in that column of the heads that share its kv head, all else is as without it."""
+    g, got, vs = q.shape[1] // ks[0].shape[1], got.copy(), [v.copy() for v in vs]
+    for b, key, column, value in broken:
+        n, m = cu[b + 1] - cu[b], len(ks[b])
+        p = m - n + np.arange(n)
+        rows = cu[b] + np.nonzero((key <= p) & (key > p - (window or m)) & (key >= first[b]))[0]
+        assert len(rows)
+        mine = got[rows, :, column]
+        assert (np.isnan(mine) if np.isnan(value) else mine == value).all()
+        got[rows, :, column] = 0
+        vs[b][key, :, column] = 0
+        vs[b][:, :, column] = np.where(np.isfinite(vs[b][:, :, column]), vs[b][:, :, column], 0)
+    for b in range(len(cu) - 1):
+        n, m = cu[b + 1] - cu[b], len(ks[b])
+        p, at = (m - n + np.arange(n))[:, None], np.arange(m)[None]
+        seen = (at <= p) & (at > p - (window or m)) & (at >= first[b])
+        for h in range(q.shape[1]):
+            want, spread, size = exact_attention(q[cu[b]:cu[b + 1], h], ks[b][:, h // g], vs[b][:, h // g], seen, scale)
+            mine = got[cu[b]:cu[b + 1], h].copy()
+            for c, key, column, _ in broken:
+                if c == b:
+                    hit = seen[:, key]
+                    want[hit, column], spread[hit, column], mine[hit, column] = 0, 0, 0
+            close(mine, want, spread, size, E[kind] if kind != kx.F32 else 0, kind)
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("heads,kv_heads,hs,page,window", [
+    (4, 2, 32, 0, 0), (7, 1, 64, 0, 90), (8, 2, 128, 16, 0), (6, 2, 64, 24, 90), (4, 4, 32, 5, 200), (3, 1, 128, 7, 40)])
+def test_prompt_values_that_are_not_finite(kind, heads, kv_heads, hs, page, window):
+    """A NaN and infinities in single columns, in tiles of which some rows see a part; pages that are not there hold NaN, and so
+    does the page that stands in for them."""
+    rng = np.random.default_rng(heads + hs + page)
+    new, lens = [330, 40, 129], [330, 210, 300] if page else [330, 40, 129]
+    cu = np.cumsum([0] + new)
+    cache = Cache(rng, lens, kv_heads, hs, page or 16, kind)
+    broken = [(0, 100, 3, np.nan), (0, 131, 9, np.inf), (0, 300, 5, -np.inf), (2, lens[2] - 1, 0, np.nan), (1, lens[1] - 3, 7, np.inf)]
+    q = rounded(rng.standard_normal((cu[-1], heads, hs)).astype(np.float32), kind)
+    vs, first = [v.copy() for v in cache.v], [0, 0, 0]
+    for b, key, column, value in broken:
+        vs[b][key, :, column] = value
+    if not page:
+        got = kx.prompt_attention(q, cu, np.concatenate(cache.k), np.concatenate(vs), window=window, kind=kind)
+    else:
+        pages, free = cache.pool.shape[0], int(cache.spare[0])
+        key, value = (np.full(cache.pool.shape, np.nan, np.float32) for _ in range(2))
+        # page 0, which stands in for those that are not there, is one that nobody has
+        moved = np.where(cache.table == 0, free, np.where(cache.table == free, 0, cache.table))
+        for b, n in enumerate(lens):
+            for t in range(n):
+                at = moved[b, t // page], t % page
+                key[at], value[at] = cache.k[b][t], vs[b][t]
+        for b in (1, 2):
+            gone = (lens[b] - new[b]) // 2 // page
+            moved[b, :gone] = -1
+            first[b] = gone * page
+        assert pages == len(key) and np.isnan(value[0]).all()
+        got = kx.prompt_attention(q, cu, pool=kx.PagePool(key, value, kind), table=moved, seq_lens=lens, window=window, kind=kind)
+    check_around(q, cu, cache.k, vs, got, kind, 1 / np.sqrt(hs), window, first, broken)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_prompt_values_that_are_not_finite_cost_little(paged):
+    """One broken value does not hold up its batch: only a tile that is partly seen is taken key by key, which adds less than this
+    call's own time.  (Pairs of a row and a head computed anew, one by one, took 200 times as long: the limit lies between.)"""
+    rng = np.random.default_rng(3)
+    n, heads, kv_heads, hs, page = 2048, 32, 8, 128, 16
+    q, k, v = (kx.to_kind(rng.standard_normal((n, m, hs)).astype(np.float32), kx.BF16) for m in (heads, kv_heads, kv_heads))
+    cu, lens = kx.Buf.from_numpy(np.array([0, n], np.int32)), kx.Buf.from_numpy(np.array([n], np.int32))
+    dq, out = kx.Buf.from_numpy(q), kx.Buf.zeros(q.shape, np.uint16)
+    table = np.arange(n // page, dtype=np.int32)[None]
+    took = []
+    for broken in (False, True):
+        if broken and paged:
+            v[:page], table = 0x7FC0, table.copy()
+            table[0, :20] = -1
+        elif broken:
+            v[n - 40, :, 3] = 0x7FC0
+        dk, dv, dt = (kx.Buf.from_numpy(a) for a in (k, v, table))
+        kv = kx.PagedKv(type=kx.BF16, kv_head_num=kv_heads, head_size=hs, page_size=page, num_pages=n // page,
+                        table_pages=n // page, batch=1, key=dk.ptr, value=dv.ptr, page_stride=page * kv_heads * hs,
+                        row_stride=kv_heads * hs, head_stride=hs, table=dt.ptr, table_stride=n // page, seq_lens=lens.ptr)
+        d = kx.PromptAttnDesc(type=kx.BF16, head_num=heads, kv_head_num=kv_heads, head_size=hs, batch=1, q_rows=n, causal=1,
+                              scale=hs ** -0.5, q=dq.ptr, q_stride=heads * hs, out=out.ptr, out_stride=heads * hs, cu_q=cu.ptr)
+        if paged:
+            d.pages = C.addressof(kv)
+        else:
+            d.k, d.v, d.cu_k, d.k_rows, d.k_stride, d.v_stride = dk.ptr, dv.ptr, cu.ptr, n, kv_heads * hs, kv_heads * hs
+        times = []
+        for _ in range(6):
+            kx.sync()
+            start = time.perf_counter()
+            for _ in range(4):
+                kx.check(kx.lib().kx_prompt_attention(C.byref(d), None))
+            kx.sync()
+            times.append(time.perf_counter() - start)
+        took.append(min(times))
+    got = kx.from_kind(out.numpy(), kx.BF16)
+    assert np.isfinite(got[320:n - 40]).all() and np.isnan(got[n - 40:, :, 3]).all() != paged
+    assert took[1] < 20 * took[0], took
 
 
 # ------------------------------------------------------------------ sure tokens
