@@ -30,9 +30,11 @@
 // turn against that, us: a prompt of 4096 143 / 145, packed prompts 52.7 / 52.0, pieces 94.3 / 93.8.)  The running maximum follows only when it is
 // exceeded by more than 2^8: weights up to 256 have the same relative precision, and the rescaling pass is rare.
 //
-// Values that are not finite and that some pairs of a tile do not see: the edge tiles are looked through for them (1 % of a
-// prompt of 4096), and one that holds any is taken key by key when the others are done: 50 - 70 us per wave, side by side.  (Pairs
-// with such a result computed anew over all of their keys, one after the other, took 27 ms for a prompt of 4096.)
+// Values that are not finite: hidden from a pair, they meet its weight of zero all the same.  A workgroup with a result that is
+// not finite goes through its keys once more; then a tile that a wave sees in part and that holds such a value is taken key by key when
+// the others are done (50 - 70 us, all waves side by side): one NaN in a prompt of 4096 0.35 ms, 512 rows over a window
+// with pages of NaN standing in for those left behind 59 us for 34.  (Pairs with such results computed anew one by one: 27 ms and
+// 8.3 ms.  The edge tiles looked through in every call: 4 % of short prompts' time, 1 % this way.)
 #include <math.h>
 
 #include <type_traits>
@@ -188,8 +190,9 @@ __device__ __forceinline__ u32x4 read_tile(lds_vec_ptr __restrict__ p) { return 
 // NW: waves of the workgroup.  KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
 // chains of tiles and more workgroups where there are few pairs.  (Narrower heads of 16-bit types keep to 128 registers: two workgroups
 // share a CU.)
-template <typename T, int HS, int MODE, int KG, int NW>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW / 4) void prompt_attn_kernel(const PromptArgs a) {
+// CAREFUL: the second time, for values that are not finite (see above).  Returns whether that is called for, to all waves alike.
+template <typename T, int HS, int MODE, int KG, int NW, bool CAREFUL>
+__device__ __forceinline__ bool prompt_attn(const PromptArgs& a) {
   constexpr int PW = NW / KG;                    // waves of a group
   constexpr int PAIRS = PW * 32;                 // pairs of the workgroup
   constexpr int KT = pa_keys<T>();
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
   constexpr float kShift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
   constexpr int KS = HS * (int)sizeof(T) / 32;   // 32-byte steps of the first product
   static_assert(KP * KG % NW == 0 || KP * KG < NW, "");
-  __shared__ int sm_missing[PAGED ? NW : 1];
+  __shared__ int sm_missing[PAGED ? NW : 1], sm_odd[CAREFUL ? 1 : NW];
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // two buffers of KG tiles, K and V each
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef const __attribute__((address_space(3))) char* lds_bytes;
@@ -214,8 +217,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
   const int qcol = lane & 31, half = lane >> 5;
   const int kvh = blockIdx.x % a.kv_heads;
   PromptWork w;
-  if (!find_prompt<PAIRS, PAGED>(a, blockIdx.x / a.kv_heads, w)) return;
-  const int group = wave / PW;
+  if (!find_prompt<PAIRS, PAGED>(a, blockIdx.x / a.kv_heads, w)) return false;
+  const int group = KG == 1 ? 0 : wave / PW;
 
   // ---- this workgroup's and this wave's pairs, and what they see ----
   const int pairs = w.n * a.kv_mul, f0 = w.block * PAIRS;
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
         if (more) issue(t + KG, buf ^ 1, kt * RP / HALVES, (kt + 1) * RP / HALVES);
       }
       if (t + 2 * KG < t1) get_ids(t + 2 * KG);
-      bool odd = false;
+      bool left = false;  // for the end
       if (key0 + KT > full_hi || key0 < full_lo || missing) {
         // keys of the tile that are there
         auto pages_there = [&]() {
@@ -435,32 +438,34 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
             const int k = 32 * kt + 8 * (r / 4) + r % 4, at = key0 + k + 4 * half;
             if (at >= my_hi || at < my_lo || !(mine >> k & 1)) s[kt][r] = -INFINITY;
           }
-        // A value that is not finite must not meet the weight of zero of a pair that does not see it: a tile with such is left
-        // for the end.  Values of pages that are not there become zeros instead (every wave that finds some writes these
-        // ahead of its own reads; no pair sees them).
-        auto look = [&]() {
-          float sums[4] = {0.f, 0.f, 0.f, 0.f};  // 0, or NaN (0 times what is not finite)
-#pragma unroll 4
-          for (int j = 0; j < KP; ++j) {
-            const u32x4 x = read_tile((lds_vec_ptr)(base + TILEB + j * 1024 + lane * 16));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sums[e] = dot_dword<T>(x[e], 0u, sums[e]);
-          }
-          return __ballot(sums[0] + sums[1] + sums[2] + sums[3] != 0.f) != 0;
-        };
-        odd = look();
-        if (PAGED && odd) {
-          if (!missing) there = pages_there();
+        if constexpr (CAREFUL) {
+          // A value that is not finite must not meet the weight of zero of a pair that does not see it: a tile with such is left
+          // for the end.  Values of pages that are not there become zeros instead (every wave that finds some writes these
+          // ahead of its own reads; no pair sees them).
+          auto look = [&]() {
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};  // 0, or NaN (0 times what is not finite)
 #pragma unroll 1
-          for (int j = 0; j < KP; ++j)
-            if (!(there >> (j * RPP + lane / CH) & 1))
-              *(__attribute__((address_space(3))) u32x4*)(base + TILEB + j * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          odd = look();
-        }
-        if (odd) {
-          if (odd_last < 0) odd_first = key0;
-          odd_last = key0;
+            for (int j = 0; j < KP; ++j) {
+              const u32x4 x = read_tile((lds_vec_ptr)(base + TILEB + j * 1024 + lane * 16));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sums[e] = dot_dword<T>(x[e], 0u, sums[e]);
+            }
+            return __ballot(sums[0] + sums[1] + sums[2] + sums[3] != 0.f) != 0;
+          };
+          left = look();
+          if (PAGED && left) {
+            if (!missing) there = pages_there();
+#pragma unroll 1
+            for (int j = 0; j < KP; ++j)
+              if (!(there >> (j * RPP + lane / CH) & 1))
+                *(__attribute__((address_space(3))) u32x4*)(base + TILEB + j * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            left = look();
+          }
+          if (left) {
+            if (odd_last < 0) odd_first = key0;
+            odd_last = key0;
+          }
         }
       }
       float mx = s[0][0];
@@ -481,7 +486,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
         m = m_new;
       }
       const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
-      if (!odd) {
+      if (!left) {
 #pragma unroll
         for (int kt = 0; kt < KT / 32; ++kt) {
           float sum = 0.f;
@@ -526,59 +531,61 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  // ---- the tiles that were left: key by key, each pair with those that it sees, from memory.  A lane has half of its pair's
-  //      query and of its values ----
-  for (int key0 = odd_first; key0 <= odd_last; key0 += KG * KT) {
-    if (key0 + KT <= full_hi && key0 >= full_lo && !missing) continue;
-    // a row's byte offset; whether it is there
-    auto row_at = [&](int t, int64_t stride, bool& there) -> int64_t {
-      if constexpr (PAGED) {
-        const int page = lookup(t);
-        there = page_ok(page);
-        return paged_offset(page, t);
-      } else {
-        there = true;
-        return t * stride * (int)sizeof(T);
-      }
-    };
-    float sum = 0.f;
-    for (int j = 0; j < KP; ++j) {
-      const int t = key0 + j * RPP + lane / CH;
-      bool there;
-      const char* vr = reinterpret_cast<const char*>(vbase) + row_at(min(t, w.keys - 1), v_stride, there) + lane % CH * 16;
-      if (t >= w.keys || !there) continue;
-      const u32x4 x = *KX_CK(a, PP_V, reinterpret_cast<const u32x4*>(vr));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum = dot_dword<T>(x[e], 0u, sum);
-    }
-    if (!__ballot(sum != 0.f)) continue;
-    const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
-#pragma unroll 1
-    for (int t = max(key0, w_lo); t < min(key0 + KT, w_hi); ++t) {
-      bool there;
-      const char* kr = reinterpret_cast<const char*>(kbase) + row_at(t, k_stride, there) + 16 * half;
-      const char* vr = reinterpret_cast<const char*>(vbase) + row_at(t, v_stride, there) + 4 * half * (int)sizeof(T);
-      if (!there) continue;
-      float x = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 k4 = *KX_CK(a, PP_K, reinterpret_cast<const u32x4*>(kr + 32 * ks)), q4 = __builtin_bit_cast(u32x4, qf[ks]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x = dot_dword<T>(k4[e], q4[e], x);
-      }
-      x += __shfl_xor(x, 32);
-      const bool seen = t >= my_lo && t < my_hi;
-      const float weight = seen ? (float)(T)__builtin_amdgcn_exp2f(fmaf(x, c, -mc)) : 0.f;
-      l += half == 0 ? weight : 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v4[4];
-          load4(KX_CKN(a, PP_V, reinterpret_cast<const T*>(vr) + 32 * dt + 8 * q, 4 * sizeof(T)), v4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = seen ? fmaf(weight, v4[e], o[dt][4 * q + e]) : o[dt][4 * q + e];
+  if constexpr (CAREFUL) {
+    // ---- the tiles that were left: key by key, each pair with those that it sees, from memory.  A lane has half of its pair's
+    //      query and of its values ----
+    for (int key0 = odd_first; key0 <= odd_last; key0 += KG * KT) {
+      if (key0 + KT <= full_hi && key0 >= full_lo && !missing) continue;
+      // a row's byte offset; whether it is there
+      auto row_at = [&](int t, int64_t stride, bool& there) -> int64_t {
+        if constexpr (PAGED) {
+          const int page = lookup(t);
+          there = page_ok(page);
+          return paged_offset(page, t);
+        } else {
+          there = true;
+          return t * stride * (int)sizeof(T);
         }
+      };
+      float sum = 0.f;
+      for (int j = 0; j < KP; ++j) {
+        const int t = key0 + j * RPP + lane / CH;
+        bool there;
+        const char* vr = reinterpret_cast<const char*>(vbase) + row_at(min(t, w.keys - 1), v_stride, there) + lane % CH * 16;
+        if (t >= w.keys || !there) continue;
+        const u32x4 x = *KX_CK(a, PP_V, reinterpret_cast<const u32x4*>(vr));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = dot_dword<T>(x[e], 0u, sum);
+      }
+      if (!__ballot(sum != 0.f)) continue;
+      const float mc = (m == -INFINITY ? 0.f : m * c) - kShift;
+#pragma unroll 1
+      for (int t = max(key0, w_lo); t < min(key0 + KT, w_hi); ++t) {
+        bool there;
+        const char* kr = reinterpret_cast<const char*>(kbase) + row_at(t, k_stride, there) + 16 * half;
+        const char* vr = reinterpret_cast<const char*>(vbase) + row_at(t, v_stride, there) + 4 * half * (int)sizeof(T);
+        if (!there) continue;
+        float x = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 k4 = *KX_CK(a, PP_K, reinterpret_cast<const u32x4*>(kr + 32 * ks)), q4 = __builtin_bit_cast(u32x4, qf[ks]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = dot_dword<T>(k4[e], q4[e], x);
+        }
+        x += __shfl_xor(x, 32);
+        const bool seen = t >= my_lo && t < my_hi;
+        const float weight = seen ? (float)(T)__builtin_amdgcn_exp2f(fmaf(x, c, -mc)) : 0.f;
+        l += half == 0 ? weight : 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v4[4];
+            load4(KX_CKN(a, PP_V, reinterpret_cast<const T*>(vr) + 32 * dt + 8 * q, 4 * sizeof(T)), v4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = seen ? fmaf(weight, v4[e], o[dt][4 * q + e]) : o[dt][4 * q + e];
+          }
+      }
     }
   }
   l = xor32_sum(l);
@@ -598,61 +605,77 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW /
       *reinterpret_cast<float*>(mine + (DT * 16 + 1) * 64 * 4 + lane * 4) = l;
     }
     __syncthreads();
-    if (group > 0) return;
+    if (group == 0) {
 #pragma unroll
-    for (int g = 1; g < KG; ++g) {
-      const char* part = smem + ((g - 1) * PW + wave) * PART;
-      const float pm = *reinterpret_cast<const float*>(part + DT * 16 * 64 * 4 + lane * 4);
-      const float pl = *reinterpret_cast<const float*>(part + (DT * 16 + 1) * 64 * 4 + lane * 4);
-      const float m_new = fmaxf(m, pm);
-      // a part without a maximum holds zeros, or NaN: those stay
-      const float fa = m == m_new ? 1.f : m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
-      const float fb = pm == m_new ? 1.f : pm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm - m_new) * c);
-      l = l * fa + pl * fb;
+      for (int g = 1; g < KG; ++g) {
+        const char* part = smem + ((g - 1) * PW + wave) * PART;
+        const float pm = *reinterpret_cast<const float*>(part + DT * 16 * 64 * 4 + lane * 4);
+        const float pl = *reinterpret_cast<const float*>(part + (DT * 16 + 1) * 64 * 4 + lane * 4);
+        const float m_new = fmaxf(m, pm);
+        // a part without a maximum holds zeros, or NaN: those stay
+        const float fa = m == m_new ? 1.f : m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * c);
+        const float fb = pm == m_new ? 1.f : pm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((pm - m_new) * c);
+        l = l * fa + pl * fb;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 po = *reinterpret_cast<const f32x4*>(part + ((dt * 4 + q) * 64 + lane) * 16);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 po = *reinterpret_cast<const f32x4*>(part + ((dt * 4 + q) * 64 + lane) * 16);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = o[dt][4 * q + e] * fa + po[e] * fb;
-        }
-      m = m_new;
-    }
-  }
-  if (wf0 >= pairs) return;
-
-  // ---- results: through the wave's part of LDS to whole rows ----
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  // (with groups: where the first of the parts that this wave alone has read lies)
-  char* region = smem + wave * (KG > 1 ? (DT * 16 + 2) * 256 : 32 * ROWB);
-  static_assert((DT * 16 + 2) * 256 >= 32 * ROWB, "");
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      typedef T vec __attribute__((ext_vector_type(4)));
-      vec y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = o[dt][4 * q + e] * inv;
-        y[e] = fabsf(x) < INFINITY ? round_to<T>(x) : (T)x;  // (an infinity that is seen stays one)
+            for (int e = 0; e < 4; ++e) o[dt][4 * q + e] = o[dt][4 * q + e] * fa + po[e] * fb;
+          }
+        m = m_new;
       }
-      const int byte = (32 * dt + 8 * q + 4 * half) * (int)sizeof(T);
-      *reinterpret_cast<vec*>(region + qcol * ROWB + ((byte >> 4 ^ k_swizzle<CH>(qcol)) << 4) + (byte & 15)) = y;
-    }
-  // (a wave's LDS instructions are served in order: it reads what its own lanes wrote)
-#pragma unroll
-  for (int j = 0; j < 32 / RPP; ++j) {
-    const int r = j * RPP + lane / CH, p = lane % CH;
-    const u32x4 y = *reinterpret_cast<const u32x4*>(region + r * ROWB + ((p ^ k_swizzle<CH>(r)) << 4));
-    const int f = wf0 + r;
-    if (f < pairs) {
-      const int row = a.mul_div.page(f);
-      char* dst = a.out + ((w.q0 + row) * a.out_stride + (kvh * a.kv_mul + f - row * a.kv_mul) * HS) * (int64_t)sizeof(T) + 16 * p;
-      *KX_CKN(a, PP_OUT, reinterpret_cast<u32x4*>(dst), 16) = y;
     }
   }
+  bool odd = false;
+  if (group == 0 && wf0 < pairs) {
+    // ---- results: through the wave's part of LDS to whole rows ----
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float sum = 0.f;  // NaN if any result is not finite
+    // (with groups: where the first of the parts that this wave alone has read lies)
+    char* region = smem + wave * (KG > 1 ? (DT * 16 + 2) * 256 : 32 * ROWB);
+    static_assert((DT * 16 + 2) * 256 >= 32 * ROWB, "");
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        typedef T vec __attribute__((ext_vector_type(4)));
+        vec y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = o[dt][4 * q + e] * inv;
+          if (!CAREFUL) sum = fmaf(x, 0.f, sum);
+          y[e] = !CAREFUL || fabsf(x) < INFINITY ? round_to<T>(x) : (T)x;  // (an infinity that is seen stays one)
+        }
+        const int byte = (32 * dt + 8 * q + 4 * half) * (int)sizeof(T);
+        *reinterpret_cast<vec*>(region + qcol * ROWB + ((byte >> 4 ^ k_swizzle<CH>(qcol)) << 4) + (byte & 15)) = y;
+      }
+    odd = __ballot(sum != 0.f) != 0;
+    // (a wave's LDS instructions are served in order: it reads what its own lanes wrote)
+#pragma unroll
+    for (int j = 0; j < 32 / RPP; ++j) {
+      const int r = j * RPP + lane / CH, p = lane % CH;
+      const u32x4 y = *reinterpret_cast<const u32x4*>(region + r * ROWB + ((p ^ k_swizzle<CH>(r)) << 4));
+      const int f = wf0 + r;
+      if (f < pairs) {
+        const int row = a.mul_div.page(f);
+        char* dst = a.out + ((w.q0 + row) * a.out_stride + (kvh * a.kv_mul + f - row * a.kv_mul) * HS) * (int64_t)sizeof(T) + 16 * p;
+        *KX_CKN(a, PP_OUT, reinterpret_cast<u32x4*>(dst), 16) = y;
+      }
+    }
+  }
+  if constexpr (CAREFUL) return false;
+  if (lane == 0) sm_odd[wave] = odd;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < NW; ++v) odd |= sm_odd[v] != 0;
+  return __builtin_amdgcn_readfirstlane(odd);
+}
+
+template <typename T, int HS, int MODE, int KG, int NW>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW / 4) void prompt_attn_kernel(const PromptArgs a) {
+  if (__builtin_expect(prompt_attn<T, HS, MODE, KG, NW, false>(a), false)) prompt_attn<T, HS, MODE, KG, NW, true>(a);
 }
 
 // the two buffers; the rows of the results pass through the same place
