@@ -17,9 +17,10 @@
 // value per lane and the weights are already the B operand of O^T = V^T P^T; the A operand V^T comes out of row-major V by
 // transposing LDS reads (16-bit types), or one element per lane (fp32).
 //
-// Reached: 1.0 PFLOP/s on a prompt of 4096 (32 heads over 8, 128 wide, bf16: 135 us), at 2.0 GHz: the chip's power, which holds
-// a library product of 8192 x 8192 x 8192 to 1.09 PFLOP/s as well.  Half the cycles are matrix instructions and half vector
-// ones there.  Tried and no faster: the two waves of a SIMD half a step apart (150 us), the next scores and the last
+// Reached: 1.0 PFLOP/s on a prompt of 4096 (32 heads over 8, 128 wide, bf16: 134 us), where a library product of 8192 x 8192 x
+// 8192 reaches 1.09.  The clock falls to 2.0 GHz there (2.3 and more in the other kernels of batched serving), and matrix
+// instructions take 51 % and vector ones 47 % of the cycles that a CU is busy (64-wide prompts: 30 and 68 %; pieces over pages:
+// 34 and 41 %).  Tried and no faster: the two waves of a SIMD half a step apart (150 us), the next scores and the last
 // second product between a wave's vector instructions (143, with spills), waiting later for the LDS-DMA (the same), two
 // workgroups of four waves and 32-key tiles per CU (154).
 // A workgroup takes 7 us beside its tiles (lengths, pages and first tiles 4, joining and storing 2).
