@@ -654,7 +654,7 @@ int kx_paged_write(const kx_paged_write_desc* desc, void* stream);
  * in fp32 arithmetic; zeros where no position is seen.  (An infinity among the seen keys and values may give NaN
  * where the formula has a limit; what is not seen may hold anything.)  q and out rows of head_num * head_size at their
  * strides (elements, multiples of 16 bytes), of type q_type: KX_F32 over any cache, KX_F16 / KX_BF16 over
- * a cache of the same type.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
+ * a cache of the same type; out may be q, at the same stride.  `workspace` (256-byte aligned) of kx_paged_decode_workspace_bytes() bytes
  * must be ZERO before its first use and is left ready for the next call by every call; calls that
  * share one must not overlap in time (kx_attn_workspace_reset's rule: after an aborted launch clear it again).
  * One workspace may serve calls of any sizes and those of kx_token_logprobs, but of no other entry.  scale is finite.
@@ -682,7 +682,7 @@ int kx_paged_decode(const kx_paged_decode_desc* desc, void* stream);
  * batch + 1 non-decreasing entries each; cu_k may be cu_q), or with `pages` (host pointer; k, v, cu_k NULL then) positions 0 ..
  * seq_lens[b]-1 of the pages.  The last query row stands at the last key: row i of n at position
  * p = (keys - n) + i; causal: it sees the keys t <= p, with window > 0 (causal only) of these t > p - window.
- * A row that sees nothing gets zeros; rows of no sequence are left alone.  All of one type
+ * A row that sees nothing gets zeros; rows of no sequence are left alone; out may be q, at the same stride.  All of one type
  * (KX_F16 / KX_BF16: matrix-core products of that type with fp32 sums and softmax, probabilities
  * rounded to it for the second product and for their sum, so that a result lies among the values that it is a mean of;
  * KX_F32: fp32 throughout).  (As in decode, an infinity among the seen keys and values may give NaN, and a sum of weighted

@@ -191,9 +191,11 @@ __device__ __forceinline__ u32x4 read_tile(lds_vec_ptr __restrict__ p) { return 
 // NW: waves of the workgroup.  KG: groups of waves that share the pairs and take every KG-th tile of the keys, joined in LDS at the end: shorter
 // chains of tiles and more workgroups where there are few pairs.  (Narrower heads of 16-bit types keep to 128 registers: two workgroups
 // share a CU.)
-// CAREFUL: the second time, for values that are not finite (see above).  Returns whether that is called for, to all waves alike.
+// CAREFUL: the second time, for values that are not finite (see above).  A wave whose results all are has stored them the first time;
+// the others (`odd`) do so now, from queries that are still whole where the results lie over them.  Returns whether a second time
+// is called for, to all waves alike.
 template <typename T, int HS, int MODE, int KG, int NW, bool CAREFUL>
-__device__ __forceinline__ bool prompt_attn(const PromptArgs& a) {
+__device__ __forceinline__ bool prompt_attn(const PromptArgs& a, bool& odd) {
   constexpr int PW = NW / KG;                    // waves of a group
   constexpr int PAIRS = PW * 32;                 // pairs of the workgroup
   constexpr int KT = pa_keys<T>();
@@ -629,7 +631,6 @@ __device__ __forceinline__ bool prompt_attn(const PromptArgs& a) {
       }
     }
   }
-  bool odd = false;
   if (group == 0 && wf0 < pairs) {
     // ---- results: through the wave's part of LDS to whole rows ----
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -652,14 +653,14 @@ __device__ __forceinline__ bool prompt_attn(const PromptArgs& a) {
         const int byte = (32 * dt + 8 * q + 4 * half) * (int)sizeof(T);
         *reinterpret_cast<vec*>(region + qcol * ROWB + ((byte >> 4 ^ k_swizzle<CH>(qcol)) << 4) + (byte & 15)) = y;
       }
-    odd = __ballot(sum != 0.f) != 0;
+    if (!CAREFUL) odd = __ballot(sum != 0.f) != 0;
     // (a wave's LDS instructions are served in order: it reads what its own lanes wrote)
 #pragma unroll
     for (int j = 0; j < 32 / RPP; ++j) {
       const int r = j * RPP + lane / CH, p = lane % CH;
       const u32x4 y = *reinterpret_cast<const u32x4*>(region + r * ROWB + ((p ^ k_swizzle<CH>(r)) << 4));
       const int f = wf0 + r;
-      if (f < pairs) {
+      if (f < pairs && odd == CAREFUL) {
         const int row = a.mul_div.page(f);
         char* dst = a.out + ((w.q0 + row) * a.out_stride + (kvh * a.kv_mul + f - row * a.kv_mul) * HS) * (int64_t)sizeof(T) + 16 * p;
         *KX_CKN(a, PP_OUT, reinterpret_cast<u32x4*>(dst), 16) = y;
@@ -669,14 +670,16 @@ __device__ __forceinline__ bool prompt_attn(const PromptArgs& a) {
   if constexpr (CAREFUL) return false;
   if (lane == 0) sm_odd[wave] = odd;
   __syncthreads();
+  int any = 0;
 #pragma unroll
-  for (int v = 0; v < NW; ++v) odd |= sm_odd[v] != 0;
-  return __builtin_amdgcn_readfirstlane(odd);
+  for (int v = 0; v < NW; ++v) any |= sm_odd[v];
+  return __builtin_amdgcn_readfirstlane(any) != 0;
 }
 
 template <typename T, int HS, int MODE, int KG, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HS <= 64 ? NW / 2 : NW / 4) void prompt_attn_kernel(const PromptArgs a) {
-  if (__builtin_expect(prompt_attn<T, HS, MODE, KG, NW, false>(a), false)) prompt_attn<T, HS, MODE, KG, NW, true>(a);
+  bool odd = false;
+  if (__builtin_expect(prompt_attn<T, HS, MODE, KG, NW, false>(a, odd), false)) prompt_attn<T, HS, MODE, KG, NW, true>(a, odd);
 }
 
 // the two buffers; the rows of the results pass through the same place

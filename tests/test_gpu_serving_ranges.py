@@ -175,6 +175,46 @@ def test_prompt_values_that_are_not_finite(kind, heads, kv_heads, hs, page, wind
     check_around(q, cu, cache.k, vs, got, kind, 1 / np.sqrt(hs), window, first, broken)
 
 
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("rows", [700, 1500])
+@pytest.mark.parametrize("broken", [False, True])
+def test_attention_over_its_own_queries(kind, rows, broken):
+    """Results that lie over the queries: the same bits as beside them, with values that are not finite as well (some waves of
+    a workgroup see those, others do not)."""
+    rng = np.random.default_rng(rows)
+    heads, kv_heads, hs = 64, 8, 128
+    q = kx.to_kind(rng.standard_normal((rows, heads, hs)).astype(np.float32), kind)
+    cache = Cache(rng, [rows], kv_heads, hs, 16, kind)
+    k, v = cache.k[0], cache.v[0].copy()
+    if broken:
+        v[[40, rows // 2, rows - 6], :, 3] = np.nan
+    dk, dv = (kx.Buf.from_numpy(kx.to_kind(a, kind)) for a in (k, v))
+    cu = kx.Buf.from_numpy(np.array([0, rows], np.int32))
+    got = []
+    for over in (False, True):
+        dq = kx.Buf.from_numpy(q)
+        out = dq if over else kx.Buf.zeros(q.shape, q.dtype)
+        d = kx.PromptAttnDesc(type=kind, head_num=heads, kv_head_num=kv_heads, head_size=hs, batch=1, q_rows=rows, k_rows=rows,
+                              causal=1, scale=hs ** -0.5, q=dq.ptr, q_stride=heads * hs, k=dk.ptr, k_stride=kv_heads * hs, v=dv.ptr,
+                              v_stride=kv_heads * hs, out=out.ptr, out_stride=heads * hs, cu_q=cu.ptr, cu_k=cu.ptr)
+        kx.check(kx.lib().kx_prompt_attention(C.byref(d), None))
+        got.append(kx.from_kind(out.numpy(q.dtype, q.shape), kind))
+    np.testing.assert_array_equal(got[0], got[1])
+    assert np.isnan(got[0][40:, :, 3]).all() == broken and np.isfinite(got[0][:40]).all() and np.isfinite(got[0][:, :, 4:]).all()
+    # single tokens, in chunks that several workgroups join
+    lens, table = kx.Buf.from_numpy(np.array([rows], np.int32)), kx.Buf.from_numpy(cache.table)
+    ws = kx.Buf.zeros(kx.lib().kx_paged_decode_workspace_bytes(1, heads, kv_heads, hs), np.uint8)
+    one = []
+    for over in (False, True):
+        dq = kx.Buf.from_numpy(q[-1:])
+        out = dq if over else kx.Buf.zeros(q[-1:].shape, q.dtype)
+        d = kx.PagedDecodeDesc(kv=cache.pool.desc(table, lens), q_type=kind, head_num=heads, scale=hs ** -0.5, q=dq.ptr,
+                               q_stride=heads * hs, out=out.ptr, out_stride=heads * hs, workspace=ws.ptr, workspace_bytes=ws.nbytes)
+        kx.check(kx.lib().kx_paged_decode(C.byref(d), None))
+        one.append(kx.from_kind(out.numpy(q.dtype, q[-1:].shape), kind))
+    np.testing.assert_array_equal(one[0], one[1])
+
+
 @pytest.mark.parametrize("paged", [False, True])
 def test_prompt_values_that_are_not_finite_cost_little(paged):
     """One broken value does not hold up its batch: only a tile that is partly seen is taken key by key, which adds less than this
