@@ -438,3 +438,74 @@ def test_prompts_that_fill_the_chip(kind, heads, hs, page):
         hidden[b][col * page:(col + 1) * page] = True
     got = kx.prompt_attention(q, cu, pool=cache.pool, table=table, seq_lens=lens, kind=kind)
     check_sample(rng, q, cu, cache.k, cache.v, got, kind, scale, 0, hidden)
+
+
+# ------------------------------------------------------------------ rows wider than what is in them
+@pytest.mark.parametrize("kind", TYPES, ids=lambda k: NAMES[k])
+@pytest.mark.parametrize("page,head_major", [(16, False), (5, True)])
+def test_strides_wider_than_rows(kind, page, head_major):
+    """q, k and v beside each other in padded rows, pages with room between their rows, tables with columns that no sequence has:
+    filed, attended as a prompt and as single tokens; the room between is left alone."""
+    rng = np.random.default_rng(page)
+    heads, kv_heads, hs, pad = 6, 2, 64, 8
+    lens = [70, 1, 33]
+    wide, es = kx.KIND_DTYPE[kind], 4 if kind == kx.F32 else 2
+    cu, rows = np.cumsum([0] + lens), sum(lens)
+    width = (heads + 2 * kv_heads) * hs + pad
+    src = rounded(rng.standard_normal((rows, width)).astype(np.float32), kind)
+    columns = -(-max(lens) // page) + 3
+    pages = max(40, 3 * columns)
+    table = np.full((3, columns + 2), 1 << 30, np.int32)
+    table[:, :columns] = rng.permutation(pages)[:3 * columns].reshape(3, columns)
+    # [page][row or head][head or row][hs] with `pad` elements behind each row of a page and of a head
+    inner = hs + pad
+    row_stride, head_stride = (inner, page * inner) if head_major else (kv_heads * inner, inner)
+    page_stride = page * kv_heads * inner + pad
+    mark = kx.to_kind(np.full(pages * page_stride, 3.0, np.float32), kind)
+    dk, dv = kx.Buf.from_numpy(mark), kx.Buf.from_numpy(mark)
+    qkv, dt = kx.Buf.from_numpy(kx.to_kind(src, kind)), kx.Buf.from_numpy(table)
+    sl, dcu = kx.Buf.from_numpy(np.array(lens, np.int32)), kx.Buf.from_numpy(cu.astype(np.int32))
+    out_stride = heads * hs + pad
+    out = kx.Buf.from_numpy(kx.to_kind(np.full((rows, out_stride), 5.0, np.float32), kind))
+    tables = rope_tables(max(lens), hs)
+    sin, cos = (kx.Buf.from_numpy(t) for t in tables)
+    kv = kx.PagedKv(type=kind, kv_head_num=kv_heads, head_size=hs, page_size=page, num_pages=pages, table_pages=columns, batch=3,
+                    key=dk.ptr, value=dv.ptr, page_stride=page_stride, row_stride=row_stride, head_stride=head_stride,
+                    table=dt.ptr, table_stride=columns + 2, seq_lens=sl.ptr)
+    w = kx.PagedWriteDesc(kv=kv, src_type=kind, rows=rows, head_num=heads, rope_variant=1, table_rows=max(lens), cu_rows=dcu.ptr,
+                          k=qkv.at(heads * hs * es), k_stride=width, v=qkv.at((heads + kv_heads) * hs * es), v_stride=width,
+                          q=qkv.ptr, q_stride=width, q_out=qkv.ptr, q_out_stride=width, sin_cache=sin.ptr, cos_cache=cos.ptr)
+    kx.check(kx.lib().kx_paged_write(C.byref(w), None))
+    now = kx.from_kind(qkv.numpy(wide, src.shape), kind)
+    np.testing.assert_array_equal(now[:, heads * hs:], src[:, heads * hs:])
+    key, value = (kx.from_kind(b.numpy(wide, mark.shape), kind) for b in (dk, dv))
+    ks, vs, filed = [], [], np.zeros(mark.shape, bool)
+    for b, n in enumerate(lens):
+        at = np.array([[table[b, t // page] * page_stride + t % page * row_stride + h * head_stride for h in range(kv_heads)]
+                       for t in range(n)])[..., None] + np.arange(hs)
+        ks.append(key[at])
+        vs.append(value[at])
+        filed[at] = True
+        np.testing.assert_array_equal(value[at].reshape(n, -1), src[cu[b]:cu[b + 1], (heads + kv_heads) * hs:-pad])
+        for t in range(n):
+            want, size = exact_rope(src[cu[b] + t, heads * hs:(heads + kv_heads) * hs].reshape(kv_heads, hs), t, tables, 1)
+            assert (np.abs(ks[b][t] - want) <= 3 * U * size + E[kind] * np.abs(want) * (1 + 2 ** -7) + 2.0 ** -25).all()
+    assert (key[~filed] == 3).all() and (value[~filed] == 3).all()
+    q = now[:, :heads * hs].reshape(rows, heads, hs)
+    p = kx.PromptAttnDesc(type=kind, head_num=heads, kv_head_num=kv_heads, head_size=hs, batch=3, q_rows=rows, causal=1,
+                          scale=0.125, q=qkv.ptr, q_stride=width, out=out.ptr, out_stride=out_stride, cu_q=dcu.ptr, pages=C.addressof(kv))
+    kx.check(kx.lib().kx_prompt_attention(C.byref(p), None))
+    got = kx.from_kind(out.numpy(wide, (rows, out_stride)), kind)
+    assert (got[:, heads * hs:] == 5).all()
+    check_prompt(q, cu, ks, vs, got[:, :heads * hs].reshape(rows, heads, hs), kind, 0.125)
+    ws = kx.Buf.zeros(kx.lib().kx_paged_decode_workspace_bytes(3, heads, kv_heads, hs), np.uint8)
+    last = qkv.numpy(wide, src.shape)[cu[1:] - 1]
+    dq, one = kx.Buf.from_numpy(last), kx.Buf.from_numpy(kx.to_kind(np.full((3, out_stride), 5.0, np.float32), kind))
+    d = kx.PagedDecodeDesc(kv=kv, q_type=kind, head_num=heads, scale=0.125, q=dq.ptr, q_stride=width, out=one.ptr,
+                           out_stride=out_stride, workspace=ws.ptr, workspace_bytes=ws.nbytes)
+    kx.check(kx.lib().kx_paged_decode(C.byref(d), None))
+    got = kx.from_kind(one.numpy(wide, (3, out_stride)), kind)
+    assert (got[:, heads * hs:] == 5).all()
+    cache = Cache.__new__(Cache)
+    cache.k, cache.v, cache.lens, cache.kind, cache.page = ks, vs, lens, kind, page
+    check_decode(cache, q[cu[1:] - 1], got[:, :heads * hs].reshape(3, heads, hs), 0, 0.125, kind)
